@@ -11,9 +11,11 @@ pids=()
 for f in $SRC; do
   o="$OBJ/$(basename "$f" .hip).o"
   if [ ! -f "$o" ] || [ "$f" -nt "$o" ] || [ "$HERE/csrc/common.h" -nt "$o" ] || [ "$HERE/csrc/cell_math.h" -nt "$o" ] || [ "$HERE/csrc/noise.h" -nt "$o" ] \
-     || [ "$HERE/../include/shivae_hip.h" -nt "$o" ]; then
+     || [ "$HERE/../include/shivae_hip.h" -nt "$o" ] || [ "$HERE/build.sh" -nt "$o" ]; then
+    # (no packed fp32 instructions: some forms of v_pk_{add,mul,fma}_f32 have given wrong results; the host pass warns that
+    # it does not know the feature)
     "$HIPCC" --offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wall -Wno-unused-function -Wno-pass-failed \
-        -c "$f" -o "$o" &
+        -Xclang -target-feature -Xclang -packed-fp32-ops -c "$f" -o "$o" &
     pids+=($!)
   fi
 done
