@@ -303,6 +303,85 @@ int shivae_presplit_weights(const float* W_dev, int N, int K, int ldw, void* ima
 int shivae_gemm_nt_presplit(int M, int N, int K, const float* A, int lda, const void* image_dev, float* C, int ldc,
                             const float* bias, const float* aux, int ldaux, int epi, int splitk, shivae_stream stream);
 
+/* ---- sequence operators -----------------------------------------------------------------------------------------
+ * A short causal convolution over time and a selective state-space scan: the recurrent scans' linear relatives, forward
+ * and backward, with states in and out and sequences of unequal length.  Time-major like everything here, channels last:
+ * a tensor [T][B][D] is addressed as t * st + b * sb + d (strides in ELEMENTS, channel stride 1), so batch-major storage
+ * is the same call with other strides.  x, y, u, dt, z, B, C, dy and their gradients have the element type `dtype`;
+ * parameters, scan states and the parameters' gradients are fp32, and so is all arithmetic.  No counterpart in the
+ * reference.
+ *   lengths_dev [B] int32 or NULL: sequence b has its first lengths[b] rows (clamped to 0..T).  Rows behind are neither
+ *   read nor of influence; in outputs and gradients they are 0.  A state that comes out is the one behind the last row
+ *   of the sequence (of an empty sequence: the state that came in).
+ * Output and gradient buffers are overwritten, all results are independent of scheduling (no atomics). */
+enum { SHIVAE_F32 = 0, SHIVAE_BF16 = 1, SHIVAE_F16 = 2 };
+
+/* y[t] = act(bias + sum_j weight[j] x[t-W+1+j]); rows in front of x are the state's. */
+typedef struct {
+    int T, B, D;
+    int W;                /* taps, 2..4 */
+    int dtype;            /* SHIVAE_F32 .. */
+    int silu;             /* 1: act(v) = v sigmoid(v), 0: none */
+    const void* x;        /* [T][B][D] */
+    int64_t x_st, x_sb;
+    const float* weight;  /* [W][D], weight[W-1] meets the newest row */
+    const float* bias;    /* [D] or NULL */
+    const void* state;    /* [W-1][B][D] dtype: the rows in front of x, or NULL (zeros) */
+    const int32_t* lengths;
+    void* y;              /* forward: [T][B][D] */
+    int64_t y_st, y_sb;
+    void* state_out;      /* forward: the last W-1 rows of each sequence, or NULL; may be `state` for T <= 16 */
+    const void* dy;       /* backward: [T][B][D] */
+    int64_t dy_st, dy_sb;
+    const void* dstate_out; /* backward: gradient of state_out, or NULL */
+    void* dx;             /* backward: [T][B][D] contiguous */
+    float* dweight;       /* [W][D] */
+    float* dbias;         /* [D]; NULL only without bias */
+    void* dstate;         /* [W-1][B][D]; NULL only without state */
+} shivae_conv_args;
+int shivae_causal_conv_fwd(const shivae_conv_args* args, shivae_stream stream);
+size_t shivae_causal_conv_bwd_ws(const shivae_conv_args* args); /* device bytes, 0 on bad arguments */
+int shivae_causal_conv_bwd(const shivae_conv_args* args, void* ws_dev, size_t ws_bytes, shivae_stream stream);
+
+/* Per channel d (group g = d / (D / G)) and state n:
+ *   s = softplus(dt + dt_bias) (or dt + dt_bias);  h[n] = exp(s A[n]) h[n] + s u B[n]
+ *   y = (sum_n C[n] h[n] + Dp u) * silu(z) */
+typedef struct {
+    int T, B, D;
+    int N;                /* states per channel, 1..64 */
+    int G;                /* groups of channels that share B and C; divides D */
+    int dtype;
+    int softplus;
+    const void *u, *dt, *z;         /* [T][B][D]; z NULL: no gate */
+    int64_t u_st, u_sb, dt_st, dt_sb, z_st, z_sb;
+    const void *Bm, *Cm;            /* [T][B][G][N], state stride 1 */
+    int64_t B_st, B_sb, B_sg, C_st, C_sb, C_sg;
+    const float* A;       /* [N][D] */
+    const float* Dp;      /* [D] or NULL */
+    const float* dt_bias; /* [D] or NULL */
+    const float* state;   /* [B][N][D] or NULL (zeros) */
+    const int32_t* lengths;
+    void* y;              /* forward: [T][B][D] */
+    int64_t y_st, y_sb;
+    float* state_out;     /* forward: [B][N][D] or NULL; may be `state` for T <= 16 */
+    float* ckpt;          /* forward: written if not NULL, backward: read: the states in front of every
+                             SHIVAE_SCAN_CKPT-th row, [ceil(T / SHIVAE_SCAN_CKPT)][B][N][D] */
+    const void* dy;       /* backward */
+    int64_t dy_st, dy_sb;
+    const float* dstate_out; /* backward: [B][N][D] or NULL */
+    void *du, *ddt, *dz;  /* [T][B][D] contiguous; dz NULL only without z */
+    void *dB, *dC;        /* [T][B][G][N] contiguous */
+    float *dA, *dDp, *ddt_bias; /* [N][D], [D], [D]; the last two NULL only without Dp / dt_bias */
+    float* dstate;        /* [B][N][D] or NULL */
+} shivae_ssm_args;
+#define SHIVAE_SCAN_CKPT 16
+/* The forward splits the time axis where B * D alone cannot fill the card; ws holds the pieces' states
+ * (shivae_selective_scan_fwd_ws bytes, 0 where nothing is split).  With T = 1 the call is the single-token step. */
+size_t shivae_selective_scan_fwd_ws(const shivae_ssm_args* args);
+int shivae_selective_scan_fwd(const shivae_ssm_args* args, void* ws_dev, size_t ws_bytes, shivae_stream stream);
+size_t shivae_selective_scan_bwd_ws(const shivae_ssm_args* args);
+int shivae_selective_scan_bwd(const shivae_ssm_args* args, void* ws_dev, size_t ws_bytes, shivae_stream stream);
+
 /* ---- optimiser ------------------------------------------------------------------------------ */
 int shivae_zero(float* buf_dev, int64_t n, shivae_stream stream);
 /* sum of squares of a flat buffer -> *out_dev (overwritten); scratch_dev: >= 1024 floats */

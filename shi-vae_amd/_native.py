@@ -37,13 +37,35 @@ SYMBOLS = ["shivae_last_error", "shivae_version", "shivae_init", "shivae_plan_se
            "shivae_sample_prior", "shivae_plan_set_noise_seed", "shivae_noise_fill", "shivae_get_output", "shivae_output_width", "shivae_get_persum", "shivae_heter_nll", "shivae_mc_impute", "shivae_kl_terms",
            "shivae_reparam_fwd", "shivae_reparam_bwd", "shivae_gemm", "shivae_zero", "shivae_sqnorm",
            "shivae_clip_adam", "shivae_scale_transform", "shivae_scale_inverse", "shivae_profile_start", "shivae_profile_active",
-           "shivae_profile_stop", "shivae_debug_gemm_stamps"]
+           "shivae_profile_stop", "shivae_debug_gemm_stamps", "shivae_causal_conv_fwd", "shivae_causal_conv_bwd_ws",
+           "shivae_causal_conv_bwd", "shivae_selective_scan_fwd_ws", "shivae_selective_scan_fwd",
+           "shivae_selective_scan_bwd_ws", "shivae_selective_scan_bwd"]
+SCAN_CKPT = 16  # SHIVAE_SCAN_CKPT
 
 
 class Config(C.Structure):
     _fields_ = [("T", C.c_int), ("B", C.c_int), ("H", C.c_int), ("Z", C.c_int), ("K", C.c_int),
                 ("n_attr", C.c_int), ("attr_type", C.POINTER(C.c_int)), ("attr_nclass", C.POINTER(C.c_int)),
                 ("learn_std", C.c_int), ("chunk_rows", C.c_int)]
+
+
+def _fields(spec):
+    """Structure fields from "type name ..." lines: i int, q int64, p pointer."""
+    kind = {"i": C.c_int, "q": C.c_int64, "p": C.c_void_p}
+    return [(name, kind[line.split()[0]]) for line in spec for name in line.split()[1:]]
+
+
+class ConvArgs(C.Structure):
+    """shivae_conv_args."""
+    _fields_ = _fields(["i T B D W dtype silu", "p x", "q x_st x_sb", "p weight bias state lengths y", "q y_st y_sb", "p state_out dy",
+                        "q dy_st dy_sb", "p dstate_out dx dweight dbias dstate"])
+
+
+class SsmArgs(C.Structure):
+    """shivae_ssm_args."""
+    _fields_ = _fields(["i T B D N G dtype softplus", "p u dt z", "q u_st u_sb dt_st dt_sb z_st z_sb", "p Bm Cm",
+                        "q B_st B_sb B_sg C_st C_sb C_sg", "p A Dp dt_bias state lengths y", "q y_st y_sb", "p state_out ckpt dy",
+                        "q dy_st dy_sb", "p dstate_out du ddt dz dB dC dA dDp ddt_bias dstate"])
 
 
 class ShiVAENativeError(RuntimeError):
@@ -118,6 +140,14 @@ def lib():
     L.shivae_scale_transform.argtypes = [vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, ci, vp]
     L.shivae_scale_inverse.argtypes = [vp, vp, ci, ci, ci, ci, vp, vp, vp, ci, vp]
     L.shivae_debug_gemm_stamps.argtypes = [vp]
+    L.shivae_causal_conv_fwd.argtypes = [vp, vp]
+    L.shivae_causal_conv_bwd_ws.argtypes = [vp]
+    L.shivae_causal_conv_bwd_ws.restype = C.c_size_t
+    L.shivae_causal_conv_bwd.argtypes = [vp, vp, C.c_size_t, vp]
+    for f in ("fwd", "bwd"):
+        getattr(L, "shivae_selective_scan_%s_ws" % f).argtypes = [vp]
+        getattr(L, "shivae_selective_scan_%s_ws" % f).restype = C.c_size_t
+        getattr(L, "shivae_selective_scan_" + f).argtypes = [vp, vp, C.c_size_t, vp]
     L.shivae_profile_start.argtypes = []
     L.shivae_profile_active.argtypes = []
     L.shivae_profile_stop.argtypes = [C.POINTER(C.c_double), ci]
