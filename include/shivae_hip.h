@@ -382,6 +382,33 @@ int shivae_selective_scan_fwd(const shivae_ssm_args* args, void* ws_dev, size_t 
 size_t shivae_selective_scan_bwd_ws(const shivae_ssm_args* args);
 int shivae_selective_scan_bwd(const shivae_ssm_args* args, void* ws_dev, size_t ws_bytes, shivae_stream stream);
 
+/* Draw a category of each row from its logits, with one uniform number per row.  Weights w = exp((x - max) / temperature);
+ * kept are the top_k largest (equal logits: lowest index first; <= 0: all), of these the shortest lead, in that order, whose
+ * weight reaches top_p of theirs (>= 1: all), of these the ones with w >= min_p; the largest is always kept.  The token is the
+ * first index i, in index order, with sum_{kept j <= i} w_j > u * sum_{kept} w_j; temperature 0 gives the largest logit's
+ * index.  NaN logits count as -inf; a row without a logit above -inf gives -1; logits at +inf share everything.  Weights are
+ * held as multiples of 2^-43 of the largest (below 2^-44 they are 0), their sums are exact.  No counterpart in the reference
+ * (generate_heter_samples averages many draws: shivae_mc_impute). */
+#define SHIVAE_SAMPLE_MAX 1048512
+typedef struct {
+    int64_t rows;
+    int V;                /* categories, 1 .. SHIVAE_SAMPLE_MAX */
+    int dtype;
+    const void* logits;   /* [rows][V], rows ld elements apart */
+    int64_t ld;
+    const float* u;       /* [rows], in [0, 1) */
+    const float* temperature_rows; /* [rows], or NULL: `temperature` for all; likewise below */
+    const int32_t* top_k_rows;
+    const float* top_p_rows;
+    const float* min_p_rows;
+    float temperature;
+    int top_k;
+    float top_p, min_p;
+    int64_t* tokens;      /* [rows] */
+    float* logprob;       /* [rows] log of the token's share of the kept weight, or NULL */
+} shivae_sample_args;
+int shivae_sample_categories(const shivae_sample_args* args, shivae_stream stream);
+
 /* ---- optimiser ------------------------------------------------------------------------------ */
 int shivae_zero(float* buf_dev, int64_t n, shivae_stream stream);
 /* sum of squares of a flat buffer -> *out_dev (overwritten); scratch_dev: >= 1024 floats */

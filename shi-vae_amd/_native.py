@@ -39,7 +39,7 @@ SYMBOLS = ["shivae_last_error", "shivae_version", "shivae_init", "shivae_plan_se
            "shivae_clip_adam", "shivae_scale_transform", "shivae_scale_inverse", "shivae_profile_start", "shivae_profile_active",
            "shivae_profile_stop", "shivae_debug_gemm_stamps", "shivae_causal_conv_fwd", "shivae_causal_conv_bwd_ws",
            "shivae_causal_conv_bwd", "shivae_selective_scan_fwd_ws", "shivae_selective_scan_fwd",
-           "shivae_selective_scan_bwd_ws", "shivae_selective_scan_bwd"]
+           "shivae_selective_scan_bwd_ws", "shivae_selective_scan_bwd", "shivae_sample_categories"]
 SCAN_CKPT = 16  # SHIVAE_SCAN_CKPT
 
 
@@ -50,8 +50,8 @@ class Config(C.Structure):
 
 
 def _fields(spec):
-    """Structure fields from "type name ..." lines: i int, q int64, p pointer."""
-    kind = {"i": C.c_int, "q": C.c_int64, "p": C.c_void_p}
+    """Structure fields from "type name ..." lines: i int, q int64, f float, p pointer."""
+    kind = {"i": C.c_int, "f": C.c_float, "q": C.c_int64, "p": C.c_void_p}
     return [(name, kind[line.split()[0]]) for line in spec for name in line.split()[1:]]
 
 
@@ -66,6 +66,12 @@ class SsmArgs(C.Structure):
     _fields_ = _fields(["i T B D N G dtype softplus", "p u dt z", "q u_st u_sb dt_st dt_sb z_st z_sb", "p Bm Cm",
                         "q B_st B_sb B_sg C_st C_sb C_sg", "p A Dp dt_bias state lengths y", "q y_st y_sb", "p state_out ckpt dy",
                         "q dy_st dy_sb", "p dstate_out du ddt dz dB dC dA dDp ddt_bias dstate"])
+
+
+class SampleArgs(C.Structure):
+    """shivae_sample_args."""
+    _fields_ = _fields(["q rows", "i V dtype", "p logits", "q ld", "p u temperature_rows top_k_rows top_p_rows min_p_rows",
+                        "f temperature", "i top_k", "f top_p min_p", "p tokens logprob"])
 
 
 class ShiVAENativeError(RuntimeError):
@@ -144,6 +150,7 @@ def lib():
     L.shivae_causal_conv_bwd_ws.argtypes = [vp]
     L.shivae_causal_conv_bwd_ws.restype = C.c_size_t
     L.shivae_causal_conv_bwd.argtypes = [vp, vp, C.c_size_t, vp]
+    L.shivae_sample_categories.argtypes = [vp, vp]
     for f in ("fwd", "bwd"):
         getattr(L, "shivae_selective_scan_%s_ws" % f).argtypes = [vp]
         getattr(L, "shivae_selective_scan_%s_ws" % f).restype = C.c_size_t

@@ -1,0 +1,635 @@
+// Drawing a category from logits with temperature, top-k, top-p and min-p, one uniform number per row.
+//
+//   w_i = exp((x_i - max) / temperature); order = by value descending, equal values by index ascending
+//   kept: the first top_k in the order; of these the shortest lead whose weight reaches top_p of theirs; of these w >= min_p
+//   token = the first index i, in index order, with  sum_{kept j <= i} w_j > u * sum_{kept j} w_j
+//
+// Which category is drawn hangs on comparisons of long sums, and 16-bit logits have long runs of equal values, whose errors add up
+// in step.  So a weight is computed in 64 bits (a polynomial for 2^f, error below 2^-47) and held as a multiple of 2^-43 of the
+// largest: sums of these are exact, independent of order (integer LDS atomics included), and fit 63 bits for 2^20 categories.  A
+// weight below 2^-44 of the largest is 0 and is never drawn.  Order is by the logits' own bits, never by rounded quotients.
+//
+// A row is a workgroup's.  No row is sorted: top-k and top-p need the last element they keep.  A histogram of (max - x) /
+// temperature over the range that has weight (counts, or sums of weights) finds the bin it lies in; the elements of that bin -- or
+// of all bins up to it, when they are few, which leaves nothing of the row to read again -- go to a list in LDS that is sorted.  A
+// bin too full for the list (runs of equal values) is resolved by four 8-bit digits of the key instead.  Bound by the row's reads
+// for few kept elements (the row stays in L2 between the passes) and by the 64-bit exponentials, about 20 instructions each, for
+// many.
+#include "common.h"
+#include "elem.h"
+
+namespace shivae {
+
+using u64 = unsigned long long;
+
+struct SampleP {
+    shivae_sample_args a;
+};
+
+struct RowParams {
+    float temperature, top_p, min_p, u;
+    int top_k;
+};
+__device__ __forceinline__ RowParams row_params(const shivae_sample_args& a, int64_t r) {
+    RowParams q;
+    q.temperature = a.temperature_rows ? a.temperature_rows[r] : a.temperature;
+    q.top_k = a.top_k_rows ? a.top_k_rows[r] : a.top_k;
+    q.top_p = a.top_p_rows ? a.top_p_rows[r] : a.top_p;
+    q.min_p = fminf(a.min_p_rows ? a.min_p_rows[r] : a.min_p, 1.f);  // the largest is always kept
+    q.u = a.u[r];
+    if (q.top_k <= 0 || q.top_k >= a.V) q.top_k = 0;
+    return q;
+}
+
+// A logit as it is compared: NaN counts as -inf, -0 as 0.
+__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.f; }
+// Unsigned keys in the order of the values, and back.
+__device__ __forceinline__ unsigned key_of(float x) {
+    const unsigned b = __float_as_uint(x);
+    return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
+
+constexpr int kFix = 43;
+// 2^y for y <= 0: 2^f = sum (f ln 2)^k / k!, |f| <= 1/2; the first dropped term is (0.3466)^12 / 12! = 6e-15.
+__device__ __forceinline__ double exp2_f64(double y, int shift) {
+    const double n = rint(y), f = y - n;
+    double p = 4.4455382718708115e-10;
+    p = fma(p, f, 7.0549116208011234e-09);
+    p = fma(p, f, 1.0178086009239699e-07);
+    p = fma(p, f, 1.3215486790144309e-06);
+    p = fma(p, f, 1.5252733804059841e-05);
+    p = fma(p, f, 1.5403530393381608e-04);
+    p = fma(p, f, 1.3333558146428443e-03);
+    p = fma(p, f, 9.6181291076284772e-03);
+    p = fma(p, f, 5.5504108664821580e-02);
+    p = fma(p, f, 2.4022650695910072e-01);
+    p = fma(p, f, 6.9314718055994531e-01);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n + shift);
+}
+// The weight of x as a multiple of 2^-43: adding 2^52 rounds to whole numbers and leaves them in the mantissa.
+struct Weigh {
+    double c, top;  // log2(e) / temperature, the largest logit
+    double least;   // log2 of min_p, at least -44
+    __device__ __forceinline__ double log2w(float x) const { return ((double)x - top) * c; }
+    __device__ void set(float max, float temperature, float min_p) {
+        c = 1.4426950408889634074 / (double)temperature;
+        top = max;
+        least = min_p > 0.f ? fmax(log2((double)min_p), -44.0) : -44.0;
+    }
+    __device__ __forceinline__ bool enough(float x) const { return log2w(x) >= least; }  // min-p
+    __device__ __forceinline__ u64 fix(float x) const {
+        const double y = log2w(x);
+        if (!(y >= -44.0)) return 0;
+        return (u64)__double_as_longlong(exp2_f64(y, kFix) + 4503599627370496.0) & 0xfffffffffffffull;
+    }
+};
+
+__device__ __forceinline__ u64 shfl_u64(u64 v, int lane) { return (u64)__shfl((long long)v, lane, 64); }
+__device__ __forceinline__ u64 shfl_up_u64(u64 v, int d) { return (u64)__shfl_up((long long)v, d, 64); }
+__device__ __forceinline__ u64 wave_sum(u64 v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += (u64)__shfl_xor((long long)v, d, 64);
+    return v;
+}
+
+// ------------------------------------------------------------------------------------------------ a workgroup per row
+template <class E, int NT, int CAP, int NB>
+struct Sampler {
+    static constexpr int VE = 16 / (int)sizeof(E), NWV = NT / 64;
+    struct Shared {
+        u64 hist[NB];   // bins, or sums of 64-vector segments of the row
+        u64 list[CAP];
+        u64 wave[NWV + 1];
+        u64 found[2];
+        int count, pos;
+    };
+
+    Shared& s;
+    const int tid, lane, wv;
+    const E* p;
+    int V, off, nvec;
+    bool has_inf;  // the largest logit is +inf: +inf reads as 0, everything else as -inf
+
+    __device__ Sampler(Shared& sh, const E* row, int n) : s(sh), tid(threadIdx.x), lane(threadIdx.x & 63), wv(threadIdx.x >> 6), p(row), V(n) {
+        off = (int)(((uintptr_t)row & 15) / sizeof(E));  // vectors are aligned; the first one may start before the row
+        nvec = (n + off + VE - 1) / VE;
+        has_inf = false;
+    }
+
+    // Vector i of the row: values, -inf outside the row.
+    __device__ __forceinline__ void get(int i, float (&x)[VE]) const {
+        const int j0 = i * VE - off;
+        if (j0 >= 0 && j0 + VE <= V) {
+            const Pack<E, VE> r = *reinterpret_cast<const Pack<E, VE>*>(p + j0);
+#pragma unroll
+            for (int k = 0; k < VE; ++k) x[k] = clean(elem_f(r.v[k]));
+        } else {
+#pragma unroll
+            for (int k = 0; k < VE; ++k) x[k] = j0 + k >= 0 && j0 + k < V ? clean(elem_f(p[j0 + k])) : -INFINITY;
+        }
+        if (has_inf)
+#pragma unroll
+            for (int k = 0; k < VE; ++k) x[k] = x[k] == INFINITY ? 0.f : -INFINITY;
+    }
+
+    // Exclusive sum of v over the workgroup's threads, and the whole sum.  Ends with a barrier behind the last read.
+    __device__ u64 scan(u64 v, u64& total) {
+        u64 in = v;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const u64 o = shfl_up_u64(in, d);
+            if (lane >= d) in += o;
+        }
+        if (NWV == 1) {
+            total = shfl_u64(in, 63);
+            return in - v;
+        }
+        if (lane == 63) s.wave[wv] = in;
+        __syncthreads();
+        u64 before = 0, all = 0;
+        for (int i = 0; i < NWV; ++i) {
+            const u64 w = s.wave[i];
+            if (i < wv) before += w;
+            all += w;
+        }
+        total = all;
+        __syncthreads();
+        return before + in - v;
+    }
+
+    // The first of n items, in order, at which the running sum exceeds what goal(total) gives; -> its number (n if none), the sum in
+    // front of it in `before`.
+    template <class W, class G>
+    __device__ int first_beyond(int n, W weight, G goal, u64& before, u64& total) {
+        const int per = (n + NT - 1) / NT, i0 = min(n, tid * per), i1 = min(n, i0 + per);
+        u64 sum = 0;
+        for (int i = i0; i < i1; ++i) sum += weight(i);
+        u64 run = scan(sum, total);
+        const u64 g = goal(total);
+        if (tid == 0) {
+            s.pos = n;
+            s.found[0] = 0;
+        }
+        __syncthreads();
+        if (run <= g && run + sum > g)
+            for (int i = i0; i < i1; ++i) {
+                const u64 w = weight(i);
+                if (run + w > g) {
+                    s.pos = i;
+                    s.found[0] = run;
+                    break;
+                }
+                run += w;
+            }
+        __syncthreads();
+        const int at = s.pos;
+        before = s.found[0];
+        __syncthreads();
+        return at;
+    }
+
+    // list[0, n), padded to a power of two with zeros, into descending order.
+    __device__ void sort(int n) {
+        int m = 1;
+        while (m < n) m <<= 1;
+        for (int i = n + tid; i < m; i += NT) s.list[i] = 0;
+        __syncthreads();
+        for (int k = 2; k <= m; k <<= 1)
+            for (int j = k >> 1; j; j >>= 1) {
+                for (int i = tid; i < m / 2; i += NT) {
+                    const int a = (i & ~(j - 1)) * 2 + (i & (j - 1)), b = a + j;
+                    const u64 x = s.list[a], y = s.list[b];
+                    if ((x < y) == ((a & k) == 0)) {
+                        s.list[a] = y;
+                        s.list[b] = x;
+                    }
+                }
+                __syncthreads();
+            }
+    }
+
+    // One addition to bin b of the histogram; lanes with b < 0 have none.  Runs of equal values put a whole wave into one bin.
+    __device__ __forceinline__ void add(int b, u64 v) {
+        const u64 on = __ballot(b >= 0);
+        if (!on) return;
+        const int first = __shfl(b, __ffsll((long long)on) - 1, 64);
+        if (__ballot(b == first) == on && __popcll(on) > 8) {
+            const u64 sum = wave_sum(b >= 0 ? v : 0);
+            if (lane == 0) atomicAdd(&s.hist[first], sum);
+        } else if (b >= 0) {
+            atomicAdd(&s.hist[b], v);
+        }
+    }
+    __device__ void clear(int n) {
+        for (int i = tid; i < n; i += NT) s.hist[i] = 0;
+        __syncthreads();
+    }
+
+    u64 last;  // the last kept element's place in the order; 0: everything is kept
+    // A place in the order, as key << 32 | ~index: larger comes first.
+    __device__ __forceinline__ static u64 place(float x, int idx) { return (u64)key_of(x) << 32 | (0xffffffffu - (unsigned)idx); }
+
+    // (max - x) scaled to bins: monotone in x, so bins are in the order of the values.  NB - 1: no weight.
+    float top, bscale;
+    __device__ __forceinline__ int bin(float x) const { return x == -INFINITY ? NB - 1 : (int)fminf((top - x) * bscale, (float)(NB - 1)); }
+
+    // The element at which the running sum, in the order, over the kept elements of bin b first exceeds g (sum in front of the bin:
+    // `before`), by counts or by weights.
+    template <class W>
+    __device__ u64 resolve(int b, u64 before, u64 g, int population, W weight) {
+        if (population <= CAP) {
+            if (tid == 0) s.count = 0;
+            __syncthreads();
+            for (int i = tid; i < nvec; i += NT) {
+                float x[VE];
+                get(i, x);
+#pragma unroll
+                for (int k = 0; k < VE; ++k)
+                    if (bin(x[k]) == b && b < NB - 1) {
+                        const u64 e = place(x[k], i * VE + k - off);
+                        if (e >= last) s.list[atomicAdd(&s.count, 1)] = e;
+                    }
+            }
+            __syncthreads();
+            const int n = s.count;
+            __syncthreads();
+            sort(n);
+            u64 bf, total;
+            const int at = first_beyond(n, [&](int i) { return weight(of_key((unsigned)(s.list[i] >> 32))); }, [&](u64) { return g - before; }, bf, total);
+            const u64 e = n ? s.list[min(at, n - 1)] : last;
+            __syncthreads();
+            return e;
+        }
+        unsigned prefix = 0, mask = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            clear(256);
+            for (int i = tid; i < round_up_vec(); i += NT) {
+                float x[VE];
+                if (i < nvec) get(i, x);
+#pragma unroll
+                for (int k = 0; k < VE; ++k) {
+                    int d = -1;
+                    if (i < nvec && bin(x[k]) == b && (key_of(x[k]) & mask) == prefix && place(x[k], i * VE + k - off) >= last)
+                        d = 255 - (int)((key_of(x[k]) >> shift) & 255);
+                    add(d, d >= 0 ? weight(x[k]) : 0);
+                }
+            }
+            __syncthreads();
+            u64 bf, total;
+            const int d = min(first_beyond(256, [&](int i) { return s.hist[i]; }, [&](u64) { return g - before; }, bf, total), 255);
+            before += bf;
+            prefix |= (unsigned)(255 - d) << shift;
+            mask |= 255u << shift;
+            __syncthreads();
+        }
+        // Equal values from here on: which of them in index order
+        const float x0 = of_key(prefix);
+        const u64 w = weight(x0), nth = w ? (g - before) / w : 0;
+        u64 bf, total;
+        float xv;
+        const int idx = locate([&](float x, int i) { return (u64)(x == x0 && place(x, i) >= last); }, [&](u64) { return nth; }, bf, total, xv);
+        return place(x0, idx < 0 ? V - 1 : idx);
+    }
+    __device__ __forceinline__ int round_up_vec() const { return (nvec + 63) & ~63; }  // whole waves, for the ballots
+
+    // The first index, in index order, at which the running sum of weight(x, index) exceeds goal(total); -1 if none.  Sums of
+    // 64-vector segments first, then one wave looks into the segment.
+    template <class W, class G>
+    __device__ int locate(W weight, G goal, u64& before, u64& total, float& value) {
+        const int nseg = (nvec + 63) / 64;
+        for (int i = tid; i < nseg * 64; i += NT) {
+            float x[VE];
+            u64 sum = 0;
+            if (i < nvec) {
+                get(i, x);
+#pragma unroll
+                for (int k = 0; k < VE; ++k) sum += weight(x[k], i * VE + k - off);
+            }
+            sum = wave_sum(sum);
+            if (lane == 0) s.hist[i >> 6] = sum;
+        }
+        __syncthreads();
+        u64 g = 0;
+        const int seg = first_beyond(nseg, [&](int i) { return s.hist[i]; }, [&](u64 t) { return g = goal(t); }, before, total);
+        if (tid == 0) s.pos = -1;
+        __syncthreads();
+        if (seg < nseg && wv == 0) {
+            const int i = seg * 64 + lane;
+            float x[VE];
+            u64 w[VE], sum = 0;
+            if (i < nvec) get(i, x);
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                w[k] = i < nvec ? weight(x[k], i * VE + k - off) : 0;
+                sum += w[k];
+            }
+            u64 in = sum;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const u64 o = shfl_up_u64(in, d);
+                if (lane >= d) in += o;
+            }
+            u64 run = before + in - sum;
+            if (run <= g && run + sum > g) {
+                bool open = true;
+#pragma unroll
+                for (int k = 0; k < VE; ++k) {
+                    if (open && run + w[k] > g) {
+                        open = false;
+                        s.pos = i * VE + k - off;
+                        s.found[1] = __float_as_uint(x[k]);
+                    }
+                    run += w[k];
+                }
+            }
+        }
+        __syncthreads();
+        const int idx = s.pos;
+        value = __uint_as_float((unsigned)s.found[1]);
+        __syncthreads();
+        return idx;
+    }
+
+    __device__ void run(const RowParams& q, int64_t* token, float* logprob) {
+        // 1. the largest, lowest index first
+        u64 best = 0;
+        for (int i = tid; i < nvec; i += NT) {
+            float x[VE];
+            get(i, x);
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                const int idx = i * VE + k - off;
+                const u64 e = place(x[k], idx);
+                if (idx >= 0 && idx < V && e > best) best = e;
+            }
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) {
+            const u64 o = (u64)__shfl_xor((long long)best, d, 64);
+            best = o > best ? o : best;
+        }
+        if (NWV > 1) {
+            if (lane == 0) s.wave[wv] = best;
+            __syncthreads();
+            for (int i = 0; i < NWV; ++i) best = s.wave[i] > best ? s.wave[i] : best;
+            __syncthreads();
+        }
+        top = of_key((unsigned)(best >> 32));
+        const int arg = (int)(0xffffffffu - (unsigned)best);
+        if (top == -INFINITY || !(q.temperature > 0.f)) {
+            if (tid == 0) {
+                *token = top == -INFINITY ? -1 : arg;
+                if (logprob) *logprob = top == -INFINITY ? -INFINITY : 0.f;
+            }
+            return;
+        }
+        if (top == INFINITY) {  // the limit of ever larger logits: those at +inf share everything
+            has_inf = true;
+            top = 0.f;
+        }
+        Weigh wt;
+        wt.set(top, q.temperature, q.min_p);
+        bscale = fminf((float)(NB - 1) / (31.f * q.temperature), 1e30f);
+        last = 0;
+        const auto one = [](float) { return (u64)1; };
+        const auto fix = [&](float x) { return wt.fix(x); };
+
+        // 2. all that top-k keeps, or a small row, into the list
+        int n = -1;  // elements in the list, if it holds all candidates
+        if (q.top_k || q.top_p < 1.f) {
+            int bk = NB - 2;
+            u64 bf = 0, total = 0;
+            int pop = 0;
+            if (V > CAP && q.top_k) {
+                clear(NB);
+                for (int i = tid; i < round_up_vec(); i += NT) {
+                    float x[VE];
+                    if (i < nvec) get(i, x);
+#pragma unroll
+                    for (int k = 0; k < VE; ++k) {
+                        const int b = i < nvec ? bin(x[k]) : NB - 1;
+                        add(b < NB - 1 ? b : -1, 1);
+                    }
+                }
+                __syncthreads();
+                bk = first_beyond(NB - 1, [&](int i) { return s.hist[i]; }, [&](u64) { return (u64)q.top_k - 1; }, bf, total);
+                pop = bk < NB - 1 ? (int)s.hist[bk] : 0;
+                __syncthreads();
+            }
+            const bool cut = bk < NB - 1;  // (with fewer than top_k elements of any weight top-k keeps them all)
+            if (V <= CAP || (q.top_k && (cut ? (int64_t)bf + pop : (int64_t)total) <= CAP)) {
+                if (tid == 0) s.count = 0;
+                __syncthreads();
+                for (int i = tid; i < nvec; i += NT) {
+                    float x[VE];
+                    get(i, x);
+#pragma unroll
+                    for (int k = 0; k < VE; ++k)
+                        if (bin(x[k]) <= min(bk, NB - 2)) s.list[atomicAdd(&s.count, 1)] = place(x[k], i * VE + k - off);
+                }
+                __syncthreads();
+                n = s.count;
+                __syncthreads();
+            } else if (q.top_k && cut) {
+                last = resolve(bk, bf, (u64)q.top_k - 1, pop, one);
+            }
+        }
+        u64 before, total;
+        float xv = top;
+        int idx;
+        if (n >= 0) {
+            sort(n);
+            if (q.top_k) n = min(n, q.top_k);
+            if (q.top_p < 1.f) {
+                const int at = first_beyond(n, [&](int i) { return wt.fix(of_key((unsigned)(s.list[i] >> 32))); },
+                                            [&](u64 t) { return lead(q.top_p, t); }, before, total);
+                n = min(n, at + 1);
+            }
+            // into index order; what min-p drops goes to the end
+            for (int i = tid; i < n; i += NT) {
+                const u64 e = s.list[i];
+                const unsigned key = (unsigned)(e >> 32);
+                s.list[i] = wt.enough(of_key(key)) ? (e << 32) | key : 0;
+            }
+            __syncthreads();
+            sort(n);
+            const int at = first_beyond(n, [&](int i) { return s.list[i] ? wt.fix(of_key((unsigned)s.list[i])) : 0; },
+                                        [&](u64 t) { return draw(q.u, t); }, before, total);
+            const u64 e = s.list[min(at, n - 1)];
+            idx = (int)(0xffffffffu - (unsigned)(e >> 32));
+            xv = of_key((unsigned)e);
+        } else {
+            // 3. top-p over the row: the bin in which the lead ends
+            if (q.top_p < 1.f) {
+                clear(NB);
+                for (int i = tid; i < round_up_vec(); i += NT) {
+                    float x[VE];
+                    if (i < nvec) get(i, x);
+#pragma unroll
+                    for (int k = 0; k < VE; ++k) {
+                        int b = i < nvec ? bin(x[k]) : NB - 1;
+                        if (last && place(x[k], i * VE + k - off) < last) b = NB - 1;
+                        add(b < NB - 1 ? b : -1, b < NB - 1 ? wt.fix(x[k]) : 0);
+                    }
+                }
+                __syncthreads();
+                u64 bf, g = 0;
+                const int bp = first_beyond(NB - 1, [&](int i) { return s.hist[i]; }, [&](u64 t) { return g = lead(q.top_p, t); }, bf, total);
+                if (bp < NB - 1) {
+                    if (tid == 0) s.count = 0;
+                    __syncthreads();
+                    int c = 0;
+                    for (int i = tid; i < nvec; i += NT) {
+                        float x[VE];
+                        get(i, x);
+#pragma unroll
+                        for (int k = 0; k < VE; ++k) c += bin(x[k]) == bp;
+                    }
+                    atomicAdd(&s.count, c);
+                    __syncthreads();
+                    const int pop = s.count;
+                    __syncthreads();
+                    last = resolve(bp, bf, g, pop, fix);
+                }
+            }
+            // 4. the draw over the row
+            const float low = of_key((unsigned)(last >> 32));
+            const bool all = last == 0;
+            idx = locate(
+                [&](float x, int i) {
+                    if (!all && (x < low || (x == low && place(x, i) < last))) return (u64)0;
+                    return wt.enough(x) ? wt.fix(x) : 0;
+                },
+                [&](u64 t) { return draw(q.u, t); }, before, total, xv);
+            if (idx < 0) {
+                idx = arg;
+                xv = top;
+            }
+        }
+        if (tid == 0) {
+            *token = idx;
+            if (logprob) *logprob = (float)(wt.log2w(xv) * 0.69314718055994530942 - log(ldexp((double)total, -kFix)));
+        }
+    }
+    // Running sums are whole numbers: sum >= p * total is sum > ceil(p * total) - 1, sum > u * total is sum > floor(u * total).
+    __device__ static u64 lead(float p, u64 total) {
+        const double g = ceil(fmax((double)p, 0.0) * (double)total);
+        return g < 1.0 ? 0 : (u64)g - 1;  // (past 2^53 a double has no g - 1)
+    }
+    __device__ static u64 draw(float u, u64 total) {
+        const u64 g = (u64)(fmax((double)u, 0.0) * (double)total);
+        return g < total ? g : (total ? total - 1 : 0);
+    }
+};
+
+template <class E, int NT, int CAP, int NB>
+__global__ __launch_bounds__(NT) void sample_kernel(SampleP p) {
+    using S = Sampler<E, NT, CAP, NB>;
+    __shared__ typename S::Shared sh;
+    const int64_t r = blockIdx.x;
+    S s(sh, static_cast<const E*>(p.a.logits) + r * p.a.ld, p.a.V);
+    s.run(row_params(p.a, r), p.a.tokens + r, p.a.logprob ? p.a.logprob + r : nullptr);
+}
+
+// ------------------------------------------------------------------------------------------------ few categories
+// L lanes per row (a power of two), a lane per category.  A lane finds what precedes it in the order by looking at every other one.
+template <class E, int L>
+__global__ __launch_bounds__(256) void sample_few_kernel(SampleP p) {
+    const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+    const int j = threadIdx.x & (L - 1);
+    const bool live = r < p.a.rows;
+    const int64_t rr = live ? r : 0;
+    const RowParams q = row_params(p.a, rr);
+    float x = live && j < p.a.V ? clean(elem_f(static_cast<const E*>(p.a.logits)[rr * p.a.ld + j])) : -INFINITY;
+    float top = x;
+#pragma unroll
+    for (int d = L / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, L));
+    const float top0 = top;
+    if (top == INFINITY) {
+        x = x == INFINITY ? 0.f : -INFINITY;
+        top = 0.f;
+    }
+    Weigh wt;
+    wt.set(top, q.temperature > 0.f ? q.temperature : 1.f, q.min_p);
+    u64 w = x == -INFINITY ? 0 : wt.fix(x);
+    int before = 0;      // elements in front of this one in the order, and their weight
+    u64 weight = 0;
+    if (__any(q.top_k != 0 || q.top_p < 1.f)) {
+        for (int i = 0; i < L; ++i) {
+            const float xi = __shfl(x, i, L);
+            const u64 wi = (u64)__shfl((long long)w, i, L);
+            if (xi > x || (xi == x && i < j)) {
+                ++before;
+                weight += wi;
+            }
+        }
+        if (q.top_k && before >= q.top_k) w = 0;
+        u64 total = w;
+#pragma unroll
+        for (int d = L / 2; d; d >>= 1) total += (u64)__shfl_xor((long long)total, d, L);
+        if (q.top_p < 1.f && before > 0 && (double)weight >= fmax((double)q.top_p, 0.0) * (double)total) w = 0;
+    }
+    if (!wt.enough(x)) w = 0;
+    u64 cum = w;
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) {
+        const u64 o = (u64)__shfl_up((long long)cum, d, L);
+        if (j >= d) cum += o;
+    }
+    const u64 total = (u64)__shfl((long long)cum, L - 1, L);
+    const u64 g0 = (u64)(fmax((double)q.u, 0.0) * (double)total), g = g0 < total ? g0 : (total ? total - 1 : 0);
+    const bool greedy = !(q.temperature > 0.f);
+    const bool hit = greedy ? x == top : (cum > g && cum - w <= g);
+    // the group's first lane that hits
+    const u64 group = L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << ((threadIdx.x & 63) & ~(L - 1));
+    const u64 hits = __ballot(hit) & group;
+    if (!live) return;
+    if (top0 == -INFINITY) {
+        if (j == 0) {
+            p.a.tokens[r] = -1;
+            if (p.a.logprob) p.a.logprob[r] = -INFINITY;
+        }
+    } else if (hit && (int)(threadIdx.x & 63) == __ffsll((long long)hits) - 1) {
+        p.a.tokens[r] = j;
+        if (p.a.logprob) p.a.logprob[r] = greedy ? 0.f : (float)(wt.log2w(x) * 0.69314718055994530942 - log(ldexp((double)total, -kFix)));
+    }
+}
+
+template <class E>
+static void launch_sample(const SampleP& p, hipStream_t s) {
+    const int V = p.a.V;
+    if (V <= 64) {
+        const int L = V <= 2 ? 2 : V <= 4 ? 4 : V <= 8 ? 8 : V <= 16 ? 16 : V <= 32 ? 32 : 64;
+        const dim3 grid((unsigned)((p.a.rows * L + 255) / 256));
+        if (L == 2) hipLaunchKernelGGL((sample_few_kernel<E, 2>), grid, dim3(256), 0, s, p);
+        else if (L == 4) hipLaunchKernelGGL((sample_few_kernel<E, 4>), grid, dim3(256), 0, s, p);
+        else if (L == 8) hipLaunchKernelGGL((sample_few_kernel<E, 8>), grid, dim3(256), 0, s, p);
+        else if (L == 16) hipLaunchKernelGGL((sample_few_kernel<E, 16>), grid, dim3(256), 0, s, p);
+        else if (L == 32) hipLaunchKernelGGL((sample_few_kernel<E, 32>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((sample_few_kernel<E, 64>), grid, dim3(256), 0, s, p);
+        return;
+    }
+    const dim3 grid((unsigned)p.a.rows);
+    if (V <= 512) hipLaunchKernelGGL((sample_kernel<E, 64, 512, 64>), grid, dim3(64), 0, s, p);
+    else if (V <= 16384) hipLaunchKernelGGL((sample_kernel<E, 256, 2048, 2048>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((sample_kernel<E, 1024, 4096, 4096>), grid, dim3(1024), 0, s, p);
+}
+
+}  // namespace shivae
+
+using namespace shivae;
+
+extern "C" int shivae_sample_categories(const shivae_sample_args* args, shivae_stream stream) {
+    SV_REQUIRE(args, "sample_categories: null argument block");
+    const shivae_sample_args& a = *args;
+    SV_REQUIRE(a.rows > 0 && a.rows < (int64_t)1 << 25, "sample_categories: %lld rows, 1 to 2^25 are supported", (long long)a.rows);
+    SV_REQUIRE(a.V >= 1 && a.V <= SHIVAE_SAMPLE_MAX, "sample_categories: %d categories, 1 to %d are supported", a.V, SHIVAE_SAMPLE_MAX);
+    SV_REQUIRE(a.dtype == SHIVAE_F32 || a.dtype == SHIVAE_BF16 || a.dtype == SHIVAE_F16, "sample_categories: unknown dtype %d", a.dtype);
+    SV_REQUIRE(a.logits && a.u && a.tokens, "sample_categories: logits, u and tokens are required");
+    const SampleP p{a};
+    SV_BY_DTYPE(a.dtype, launch_sample<E>(p, static_cast<hipStream_t>(stream)));
+    SV_CHECK_HIP(hipGetLastError());
+    return SHIVAE_OK;
+}

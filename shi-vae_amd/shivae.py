@@ -27,6 +27,7 @@ import torch.nn as nn
 
 from . import _native as N
 from . import utils
+from .sampling import sample_categories
 
 print_shivae = "ELBO:{n_elbo:.3f} | NLL:{nll_loss:.3f}  KL_Q_Z:{kld_q_z:.3f}  KL_Q_S:{kld_q_s:.3f}|  " \
                "Real:{nll_real:.3f}  Pos:{nll_pos:.3f}  Bin:{nll_bin:.3f}  Cat:{nll_cat:.3f}"
@@ -708,6 +709,20 @@ class ShiVAE(nn.Module):
         N.check(N.lib().shivae_mc_impute(self._layout.h, N.ptr(P), self.p_dim, T * B, int(n_samples), int(seed),
                                          N.ptr(xhat), N.stream()))
         return xhat
+
+    @torch.no_grad()
+    def sample_categories(self, likes, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """One draw of every categorical attribute from its likelihood (of ``sample_from_prior``, ``feed2model``):
+        {name: int64 [T,B]}.  u: {name: uniforms [T,B]}, drawn on the device where it is None; the settings as in
+        :func:`shivae_amd.sample_categories` (the Monte-Carlo means of base_missvae.py:378-404 have no such draw)."""
+        self._require_gpu()
+        out = {}
+        for t in self.types_list:
+            if t['type'] == 'cat' and t['name'] in likes:
+                logits = likes[t['name']].logits
+                uu = torch.rand(logits.shape[:-1], device=logits.device) if u is None else u[t['name']]
+                out[t['name']] = sample_categories(logits, uu, temperature, top_k, top_p, min_p)
+        return out
 
     @torch.no_grad()
     def impute_mean(self, x, temp=0.01):

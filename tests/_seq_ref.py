@@ -144,11 +144,11 @@ def sample(logits, u, temperature, top_k, top_p, min_p):
         if p < 1:
             total, run, lead = sum(w[i] for i in kept), 0.0, []
             for i in kept:
-                if run < p * total:
+                if not lead or run < p * total:
                     lead.append(i)
                 run += w[i]
             kept = lead
-        kept = sorted(i for i in kept if w[i] >= m)
+        kept = sorted(i for i in kept if w[i] >= min(m, 1))
         total = sum(w[i] for i in kept)
         goal, run = float(u[r]) * total, 0.0
         for i in kept:
