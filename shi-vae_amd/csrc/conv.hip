@@ -213,27 +213,41 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvP p) {
     store_row<float, V>(part + (int64_t)W * a.D, db);
 }
 
-// out[c] = sum over k of part[k][c], c < cols; a block owns 64 columns, its four waves add every fourth partial and wave 0
-// adds the four sums: a fixed order, whatever the grid.
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64_t n, int cols, float* out0, int split, float* out1) {
+// out[c] = sum over k of part[k][c], c < cols, in a fixed order whatever the grid: a block adds `step` rows of 64 columns, its four
+// waves every fourth row, wave 0 the four sums.  With more than 64 rows a first launch adds up to 64 slices of them into `mid`.
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64_t n, int64_t step, int cols, float* out0, int split, float* out1) {
     __shared__ float acc[4][64];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    const int64_t k0 = (int64_t)blockIdx.y * step, k1 = min(n, k0 + step);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < cols)
-        for (int64_t k = wv; k < n; k += 16)
+        for (int64_t k = k0 + wv; k < k1; k += 16)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (k + 4 * q < n) s[q] += part[(k + 4 * q) * cols + c];
+                if (k + 4 * q < k1) s[q] += part[(k + 4 * q) * cols + c];
     acc[wv][lane] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
     if (wv || c >= cols) return;
     const float v = (acc[0][lane] + acc[1][lane]) + (acc[2][lane] + acc[3][lane]);
-    if (c < split) out0[c] = v;
-    else if (out1) out1[c - split] = v;
+    if (c >= split) {
+        if (out1) out1[c - split] = v;
+    } else if (out0) {
+        out0[(int64_t)blockIdx.y * cols + c] = v;
+    }
 }
 
-int launch_sum_parts(const float* part, int64_t n, int cols, float* out0, int split, float* out1, hipStream_t stream) {
-    hipLaunchKernelGGL(sum_parts_kernel, dim3(ceil_div(cols, 64)), dim3(256), 0, stream, part, n, cols, out0, split, out1);
+constexpr int kSlices = 64;
+size_t sum_parts_floats(int64_t n, int64_t cols) { return n > kSlices ? (size_t)kSlices * cols : 0; }
+
+int launch_sum_parts(const float* part, int64_t n, int cols, float* mid, float* out0, int split, float* out1, hipStream_t stream) {
+    if (n > kSlices) {
+        const int64_t step = (n + kSlices - 1) / kSlices;
+        const int slices = (int)((n + step - 1) / step);
+        hipLaunchKernelGGL(sum_parts_kernel, dim3(ceil_div(cols, 64), slices), dim3(256), 0, stream, part, n, step, cols, mid, cols, nullptr);
+        part = mid;
+        n = slices;
+    }
+    hipLaunchKernelGGL(sum_parts_kernel, dim3(ceil_div(cols, 64)), dim3(256), 0, stream, part, n, n, cols, out0, split, out1);
     SV_CHECK_HIP(hipGetLastError());
     return SHIVAE_OK;
 }
@@ -302,7 +316,8 @@ int shivae_causal_conv_fwd(const shivae_conv_args* args, shivae_stream stream) {
 size_t shivae_causal_conv_bwd_ws(const shivae_conv_args* args) {
     if (conv_check(args, "causal_conv_bwd_ws") != SHIVAE_OK) return 0;
     // (runs are shortest, and partials most, where a thread owns eight channels)
-    return (size_t)ceil_div(args->T, conv_run(*args, 8, 16)) * args->B * (args->W + 1) * args->D * sizeof(float);
+    const int64_t n = (int64_t)ceil_div(args->T, conv_run(*args, 8, 16)) * args->B, cols = (int64_t)(args->W + 1) * args->D;
+    return ((size_t)n * cols + sum_parts_floats(n, cols)) * sizeof(float);
 }
 
 int shivae_causal_conv_bwd(const shivae_conv_args* args, void* ws_dev, size_t ws_bytes, shivae_stream stream) {
@@ -324,7 +339,9 @@ int shivae_causal_conv_bwd(const shivae_conv_args* args, void* ws_dev, size_t ws
         else launch_conv<E, 1>(true, p, grid, s);
     });
     SV_CHECK_HIP(hipGetLastError());
-    return launch_sum_parts(p.part, (int64_t)p.nrun * a.B, (a.W + 1) * a.D, a.dweight, a.W * a.D, a.dbias, s);
+    const int64_t n = (int64_t)p.nrun * a.B;
+    const int cols = (a.W + 1) * a.D;
+    return launch_sum_parts(p.part, n, cols, p.part + n * cols, a.dweight, a.W * a.D, a.dbias, s);
 }
 
 }  // extern "C"

@@ -135,7 +135,7 @@ struct Sampler {
     }
 
     // Exclusive sum of v over the workgroup's threads, and the whole sum.  Ends with a barrier behind the last read.
-    __device__ u64 scan(u64 v, u64& total) {
+    __device__ __forceinline__ u64 scan(u64 v, u64& total) {
         u64 in = v;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -162,7 +162,7 @@ struct Sampler {
     // The first of n items, in order, at which the running sum exceeds what goal(total) gives; -> its number (n if none), the sum in
     // front of it in `before`.
     template <class W, class G>
-    __device__ int first_beyond(int n, W weight, G goal, u64& before, u64& total) {
+    __device__ __forceinline__ int first_beyond(int n, W weight, G goal, u64& before, u64& total) {
         const int per = (n + NT - 1) / NT, i0 = min(n, tid * per), i1 = min(n, i0 + per);
         u64 sum = 0;
         for (int i = i0; i < i1; ++i) sum += weight(i);
@@ -191,7 +191,7 @@ struct Sampler {
     }
 
     // list[0, n), padded to a power of two with zeros, into descending order.
-    __device__ void sort(int n) {
+    __device__ __forceinline__ void sort(int n) {
         int m = 1;
         while (m < n) m <<= 1;
         for (int i = n + tid; i < m; i += NT) s.list[i] = 0;
@@ -210,19 +210,60 @@ struct Sampler {
             }
     }
 
-    // One addition to bin b of the histogram; lanes with b < 0 have none.  Runs of equal values put a whole wave into one bin.
-    __device__ __forceinline__ void add(int b, u64 v) {
-        const u64 on = __ballot(b >= 0);
-        if (!on) return;
-        const int first = __shfl(b, __ffsll((long long)on) - 1, 64);
-        if (__ballot(b == first) == on && __popcll(on) > 8) {
-            const u64 sum = wave_sum(b >= 0 ? v : 0);
-            if (lane == 0) atomicAdd(&s.hist[first], sum);
-        } else if (b >= 0) {
-            atomicAdd(&s.hist[b], v);
+    // Adds every element to its bin of the histogram: bin_of(x, index) < 0 is none, value(x) what to add.  A wave whose elements
+    // all lie in one bin (runs of equal values) adds once, since additions to one address queue up.
+    template <class B, class W>
+    __device__ __forceinline__ void fill(int bins, B bin_of, W value) {
+        clear(bins);
+        for (int i = tid; i < ((nvec + 63) & ~63); i += NT) {  // whole waves, for the ballot
+            float x[VE];
+            int b[VE];
+            if (i < nvec) get(i, x);
+            bool same = true;
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                b[k] = i < nvec ? bin_of(x[k], i * VE + k - off) : -1;
+                same &= b[k] == b[0];
+            }
+            const int first = __builtin_amdgcn_readfirstlane(b[0]);
+            if (__ballot(same && b[0] == first) == ~0ull) {
+                if (first < 0) continue;
+                u64 v = 0;
+#pragma unroll
+                for (int k = 0; k < VE; ++k) v += value(x[k]);
+                v = wave_sum(v);
+                if (lane == 0) atomicAdd(&s.hist[first], v);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VE; ++k)
+                    if (b[k] >= 0) atomicAdd(&s.hist[b[k]], value(x[k]));
+            }
         }
+        __syncthreads();
     }
-    __device__ void clear(int n) {
+    // Puts the elements that take(x, index) holds into the list, in any order, as far as there is room; -> their number.
+    template <class F>
+    __device__ __forceinline__ int gather(F take) {
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+        for (int i = tid; i < nvec; i += NT) {
+            float x[VE];
+            get(i, x);
+            unsigned m = 0;
+#pragma unroll
+            for (int k = 0; k < VE; ++k) m |= take(x[k], i * VE + k - off) ? 1u << k : 0u;
+            if (!m) continue;
+            int at = atomicAdd(&s.count, __popc(m));
+#pragma unroll
+            for (int k = 0; k < VE; ++k)
+                if ((m >> k & 1) && at < CAP) s.list[at++] = place(x[k], i * VE + k - off);
+        }
+        __syncthreads();
+        const int n = s.count;
+        __syncthreads();
+        return n;
+    }
+    __device__ __forceinline__ void clear(int n) {
         for (int i = tid; i < n; i += NT) s.hist[i] = 0;
         __syncthreads();
     }
@@ -235,26 +276,18 @@ struct Sampler {
     float top, bscale;
     __device__ __forceinline__ int bin(float x) const { return x == -INFINITY ? NB - 1 : (int)fminf((top - x) * bscale, (float)(NB - 1)); }
 
+    __device__ __forceinline__ int has_weight(float x) const {  // its bin, or -1
+        const int b = bin(x);
+        return b < NB - 1 ? b : -1;
+    }
+
     // The element at which the running sum, in the order, over the kept elements of bin b first exceeds g (sum in front of the bin:
     // `before`), by counts or by weights.
     template <class W>
-    __device__ u64 resolve(int b, u64 before, u64 g, int population, W weight) {
-        if (population <= CAP) {
-            if (tid == 0) s.count = 0;
-            __syncthreads();
-            for (int i = tid; i < nvec; i += NT) {
-                float x[VE];
-                get(i, x);
-#pragma unroll
-                for (int k = 0; k < VE; ++k)
-                    if (bin(x[k]) == b && b < NB - 1) {
-                        const u64 e = place(x[k], i * VE + k - off);
-                        if (e >= last) s.list[atomicAdd(&s.count, 1)] = e;
-                    }
-            }
-            __syncthreads();
-            const int n = s.count;
-            __syncthreads();
+    __device__ __forceinline__ u64 resolve(int b, u64 before, u64 g, W weight) {
+        const auto in = [&](float x, int i) { return bin(x) == b && place(x, i) >= last; };
+        const int n = gather(in);
+        if (n <= CAP) {
             sort(n);
             u64 bf, total;
             const int at = first_beyond(n, [&](int i) { return weight(of_key((unsigned)(s.list[i] >> 32))); }, [&](u64) { return g - before; }, bf, total);
@@ -263,26 +296,14 @@ struct Sampler {
             return e;
         }
         unsigned prefix = 0, mask = 0;
+#pragma unroll 1
         for (int shift = 24; shift >= 0; shift -= 8) {
-            clear(256);
-            for (int i = tid; i < round_up_vec(); i += NT) {
-                float x[VE];
-                if (i < nvec) get(i, x);
-#pragma unroll
-                for (int k = 0; k < VE; ++k) {
-                    int d = -1;
-                    if (i < nvec && bin(x[k]) == b && (key_of(x[k]) & mask) == prefix && place(x[k], i * VE + k - off) >= last)
-                        d = 255 - (int)((key_of(x[k]) >> shift) & 255);
-                    add(d, d >= 0 ? weight(x[k]) : 0);
-                }
-            }
-            __syncthreads();
+            fill(256, [&](float x, int i) { return in(x, i) && (key_of(x) & mask) == prefix ? 255 - (int)((key_of(x) >> shift) & 255) : -1; }, weight);
             u64 bf, total;
             const int d = min(first_beyond(256, [&](int i) { return s.hist[i]; }, [&](u64) { return g - before; }, bf, total), 255);
             before += bf;
             prefix |= (unsigned)(255 - d) << shift;
             mask |= 255u << shift;
-            __syncthreads();
         }
         // Equal values from here on: which of them in index order
         const float x0 = of_key(prefix);
@@ -292,12 +313,11 @@ struct Sampler {
         const int idx = locate([&](float x, int i) { return (u64)(x == x0 && place(x, i) >= last); }, [&](u64) { return nth; }, bf, total, xv);
         return place(x0, idx < 0 ? V - 1 : idx);
     }
-    __device__ __forceinline__ int round_up_vec() const { return (nvec + 63) & ~63; }  // whole waves, for the ballots
 
     // The first index, in index order, at which the running sum of weight(x, index) exceeds goal(total); -1 if none.  Sums of
     // 64-vector segments first, then one wave looks into the segment.
     template <class W, class G>
-    __device__ int locate(W weight, G goal, u64& before, u64& total, float& value) {
+    __device__ __forceinline__ int locate(W weight, G goal, u64& before, u64& total, float& value) {
         const int nseg = (nvec + 63) / 64;
         for (int i = tid; i < nseg * 64; i += NT) {
             float x[VE];
@@ -352,7 +372,7 @@ struct Sampler {
         return idx;
     }
 
-    __device__ void run(const RowParams& q, int64_t* token, float* logprob) {
+    __device__ __forceinline__ void run(const RowParams& q, int64_t* token, float* logprob) {
         // 1. the largest, lowest index first
         u64 best = 0;
         for (int i = tid; i < nvec; i += NT) {
@@ -400,41 +420,15 @@ struct Sampler {
         int n = -1;  // elements in the list, if it holds all candidates
         if (q.top_k || q.top_p < 1.f) {
             int bk = NB - 2;
-            u64 bf = 0, total = 0;
-            int pop = 0;
+            u64 bf = 0, total = 0, upto = V;
             if (V > CAP && q.top_k) {
-                clear(NB);
-                for (int i = tid; i < round_up_vec(); i += NT) {
-                    float x[VE];
-                    if (i < nvec) get(i, x);
-#pragma unroll
-                    for (int k = 0; k < VE; ++k) {
-                        const int b = i < nvec ? bin(x[k]) : NB - 1;
-                        add(b < NB - 1 ? b : -1, 1);
-                    }
-                }
-                __syncthreads();
+                fill(NB, [&](float x, int) { return has_weight(x); }, one);
                 bk = first_beyond(NB - 1, [&](int i) { return s.hist[i]; }, [&](u64) { return (u64)q.top_k - 1; }, bf, total);
-                pop = bk < NB - 1 ? (int)s.hist[bk] : 0;
-                __syncthreads();
+                // (fewer than top_k elements of any weight: top-k keeps them all)
+                upto = bk < NB - 1 ? bf + s.hist[bk] : total;
             }
-            const bool cut = bk < NB - 1;  // (with fewer than top_k elements of any weight top-k keeps them all)
-            if (V <= CAP || (q.top_k && (cut ? (int64_t)bf + pop : (int64_t)total) <= CAP)) {
-                if (tid == 0) s.count = 0;
-                __syncthreads();
-                for (int i = tid; i < nvec; i += NT) {
-                    float x[VE];
-                    get(i, x);
-#pragma unroll
-                    for (int k = 0; k < VE; ++k)
-                        if (bin(x[k]) <= min(bk, NB - 2)) s.list[atomicAdd(&s.count, 1)] = place(x[k], i * VE + k - off);
-                }
-                __syncthreads();
-                n = s.count;
-                __syncthreads();
-            } else if (q.top_k && cut) {
-                last = resolve(bk, bf, (u64)q.top_k - 1, pop, one);
-            }
+            if (upto <= CAP) n = gather([&](float x, int) { return bin(x) <= min(bk, NB - 2); });
+            else if (q.top_k && bk < NB - 1) last = resolve(bk, bf, (u64)q.top_k - 1, one);
         }
         u64 before, total;
         float xv = top;
@@ -463,36 +457,10 @@ struct Sampler {
         } else {
             // 3. top-p over the row: the bin in which the lead ends
             if (q.top_p < 1.f) {
-                clear(NB);
-                for (int i = tid; i < round_up_vec(); i += NT) {
-                    float x[VE];
-                    if (i < nvec) get(i, x);
-#pragma unroll
-                    for (int k = 0; k < VE; ++k) {
-                        int b = i < nvec ? bin(x[k]) : NB - 1;
-                        if (last && place(x[k], i * VE + k - off) < last) b = NB - 1;
-                        add(b < NB - 1 ? b : -1, b < NB - 1 ? wt.fix(x[k]) : 0);
-                    }
-                }
-                __syncthreads();
+                fill(NB, [&](float x, int i) { return last && place(x, i) < last ? -1 : has_weight(x); }, fix);
                 u64 bf, g = 0;
                 const int bp = first_beyond(NB - 1, [&](int i) { return s.hist[i]; }, [&](u64 t) { return g = lead(q.top_p, t); }, bf, total);
-                if (bp < NB - 1) {
-                    if (tid == 0) s.count = 0;
-                    __syncthreads();
-                    int c = 0;
-                    for (int i = tid; i < nvec; i += NT) {
-                        float x[VE];
-                        get(i, x);
-#pragma unroll
-                        for (int k = 0; k < VE; ++k) c += bin(x[k]) == bp;
-                    }
-                    atomicAdd(&s.count, c);
-                    __syncthreads();
-                    const int pop = s.count;
-                    __syncthreads();
-                    last = resolve(bp, bf, g, pop, fix);
-                }
+                if (bp < NB - 1) last = resolve(bp, bf, g, fix);
             }
             // 4. the draw over the row
             const float low = of_key((unsigned)(last >> 32));

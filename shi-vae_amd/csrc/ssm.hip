@@ -23,7 +23,8 @@
 
 namespace shivae {
 
-int launch_sum_parts(const float* part, int64_t n, int cols, float* out0, int split, float* out1, hipStream_t stream);
+size_t sum_parts_floats(int64_t n, int64_t cols);
+int launch_sum_parts(const float* part, int64_t n, int cols, float* mid, float* out0, int split, float* out1, hipStream_t stream);
 
 constexpr int TT = SHIVAE_SCAN_CKPT;  // rows per tile
 
@@ -603,7 +604,8 @@ int shivae_selective_scan_fwd(const shivae_ssm_args* args, void* ws_dev, size_t 
 
 static size_t bwd_floats(const SsmP& p) {
     const shivae_ssm_args& a = p.a;
-    return piece_floats(p) + (size_t)p.tiles * a.T * a.B * 2 * a.N + (size_t)p.np * a.B * (a.N + 2) * a.D;
+    return piece_floats(p) + (size_t)p.tiles * a.T * a.B * 2 * a.N + (size_t)p.np * a.B * (a.N + 2) * a.D +
+           sum_parts_floats((int64_t)p.np * a.B, (int64_t)std::max(a.N, 2) * a.D);
 }
 
 size_t shivae_selective_scan_bwd_ws(const shivae_ssm_args* args) {
@@ -637,8 +639,9 @@ int shivae_selective_scan_bwd(const shivae_ssm_args* args, void* ws_dev, size_t 
     SV_REQUIRE((total + 255) / 256 < (int64_t)1 << 31, "selective_scan_bwd: T * B * G * N is too large");
     SV_BY_DTYPE(a.dtype, hipLaunchKernelGGL((ssm_dbc_kernel<E>), grid, dim3(256), 0, s, p));
     SV_CHECK_HIP(hipGetLastError());
-    SV_TRY(launch_sum_parts(p.pA, (int64_t)p.np * a.B, a.N * a.D, a.dA, a.N * a.D, nullptr, s));
-    if (a.Dp || a.dt_bias) return launch_sum_parts(p.pD, (int64_t)p.np * a.B, 2 * a.D, a.dDp ? a.dDp : a.ddt_bias, a.D, a.ddt_bias, s);
+    float* mid = p.pD + (size_t)p.np * a.B * 2 * a.D;
+    SV_TRY(launch_sum_parts(p.pA, (int64_t)p.np * a.B, a.N * a.D, mid, a.dA, a.N * a.D, nullptr, s));
+    if (a.Dp || a.dt_bias) return launch_sum_parts(p.pD, (int64_t)p.np * a.B, 2 * a.D, mid, a.dDp, a.D, a.ddt_bias, s);
     return SHIVAE_OK;
 }
 
