@@ -375,8 +375,9 @@ typedef struct {
     float* dstate;        /* [B][N][D] or NULL */
 } shivae_ssm_args;
 #define SHIVAE_SCAN_CKPT 16
-/* The forward splits the time axis where B * D alone cannot fill the card; ws holds the pieces' states
- * (shivae_selective_scan_fwd_ws bytes, 0 where nothing is split).  With T = 1 the call is the single-token step. */
+/* ws_dev: 16-byte aligned device memory of at least the bytes that the _ws call names, for partial sums and the pieces of the
+ * time axis, which is split where B * D alone cannot fill the card (forward: 0 bytes where it is not split).  With T = 1 and no
+ * ckpt the forward is the single-token step. */
 size_t shivae_selective_scan_fwd_ws(const shivae_ssm_args* args);
 int shivae_selective_scan_fwd(const shivae_ssm_args* args, void* ws_dev, size_t ws_bytes, shivae_stream stream);
 size_t shivae_selective_scan_bwd_ws(const shivae_ssm_args* args);

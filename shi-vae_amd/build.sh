@@ -14,7 +14,7 @@ for f in $SRC; do
      || [ "$HERE/../include/shivae_hip.h" -nt "$o" ] || [ "$HERE/build.sh" -nt "$o" ]; then
     # (no packed fp32 instructions: some forms of v_pk_{add,mul,fma}_f32 have given wrong results; the host pass warns that
     # it does not know the feature)
-    "$HIPCC" --offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wall -Wno-unused-function -Wno-pass-failed \
+    "$HIPCC" --offload-arch=gfx950 -O3 -std=c++20 -fPIC -munsafe-fp-atomics -Wall -Wno-unused-function -Wno-pass-failed \
         -Xclang -target-feature -Xclang -packed-fp32-ops -c "$f" -o "$o" &
     pids+=($!)
   fi
