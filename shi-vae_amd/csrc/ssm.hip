@@ -118,24 +118,37 @@ __device__ __forceinline__ void put(E* base, unsigned off, E v) {
     *reinterpret_cast<E*>(reinterpret_cast<char*>(base) + off) = v;
 }
 
+// (Whole words, so that the compiler does not merge the wide load with the element loads of the other branch into element loads.)
+template <int BYTES>
+struct Words {
+    typedef unsigned T __attribute__((ext_vector_type(BYTES >= 16 ? 4 : BYTES / 4)));
+    static constexpr int n = BYTES >= 16 ? BYTES / 16 : 1;
+    T v[n];
+};
+template <>
+struct Words<2> {
+    unsigned short v[1];
+};
+// What a lane needs of B or C for a tile: S states of row (lane mod 16), as loaded.
 template <class E, int S>
 struct RowRegs {
-    float v[S];
-    // base: row tb of this group's matrix; s0: first state; rows tb + (lane mod 16), 0 at and behind tn, states 0 at and behind N
+    Pack<E, S> e;
+    // base: the tile's row 0 of this group's matrix; s0: first state; left: rows from there to the sequence's end
     __device__ __forceinline__ void load(const E* base, unsigned stb, int s0, int N, bool vec, int left, int lane) {
-        const int r = lane & 15;
-        const unsigned off = (unsigned)min(r, left - 1) * stb;
-        E e[S];
+        const unsigned off = (unsigned)min(lane & 15, left - 1) * stb;
         if (vec) {
-            const Pack<E, S> q = *reinterpret_cast<const Pack<E, S>*>(reinterpret_cast<const char*>(base + s0) + off);
-#pragma unroll
-            for (int j = 0; j < S; ++j) e[j] = q.v[j];
+            using W = Words<S * sizeof(E)>;
+            const W w = *reinterpret_cast<const W*>(reinterpret_cast<const char*>(base) + (off + (unsigned)(min(s0, N - S) * sizeof(E))));
+            __builtin_memcpy(&e, &w, sizeof(e));
         } else {
 #pragma unroll
-            for (int j = 0; j < S; ++j) e[j] = at(base + min(s0 + j, N - 1), off);
+            for (int j = 0; j < S; ++j) e.v[j] = at(base, off + (unsigned)(min(s0 + j, N - 1) * sizeof(E)));
         }
+    }
+    // as fp32; rows at and behind `left` and states at and behind N are 0
+    __device__ __forceinline__ void get(float (&v)[S], int s0, int N, int left, int lane) const {
 #pragma unroll
-        for (int j = 0; j < S; ++j) v[j] = r < left && s0 + j < N ? elem_f(e[j]) : 0.f;
+        for (int j = 0; j < S; ++j) v[j] = (lane & 15) < left && s0 + j < N ? elem_f(e.v[j]) : 0.f;
     }
 };
 
@@ -165,17 +178,6 @@ __device__ __forceinline__ float swap16_add(float x, float y) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float x) {
-    return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, false));
-}
-__device__ __forceinline__ float row16_sum(float x) {
-    x = dpp_add<0x128>(x);  // row_ror:8, 4, 2, 1
-    x = dpp_add<0x124>(x);
-    x = dpp_add<0x122>(x);
-    return dpp_add<0x121>(x);
-}
-
 template <int N, class F>
 __device__ __forceinline__ void unroll(F f) {  // f(0), f(1), ... with the number as a constant
     [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
@@ -246,12 +248,10 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
         Bm += TT * a.B_st;
         Cm += TT * a.C_st;
     };
-    float total = 0.f;
-    int left = tn - t0;  // rows from the present tile's first one
-    float* ckpt = a.ckpt && !FIRST ? a.ckpt + (int64_t)(t0 / TT) * statep + state0 : nullptr;
-    if (left > 0) request(left);
-    for (; left > 0; left -= TT) {
-        float s[4], ku[4], kz[4], v[4];
+    float total = 0.f, ku[4], kz[4], vB[S], vC[S];
+    // A tile's operands as the rows below take them, from what request() loaded.
+    auto prepare = [&](int left) {
+        float s[4];
         // (flags outside of the loops over k: a branch between them would run the four chains of dependent operations in turn)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -271,32 +271,45 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
             if (FIRST) total += s[k];
             row[4 * k + g4][lane & 15] = make_float2(s[k], in ? s[k] * ku[k] : 0.f);
         }
-        const RowRegs<E, S> vB = nB, vC = nC;
+        nB.get(vB, g4 * S, a.N, left, lane);
+        if (!FIRST) nC.get(vC, g4 * S, a.N, left, lane);
+    };
+    int left = tn - t0;  // rows from the present tile's first one
+    float* ckpt = a.ckpt && !FIRST ? a.ckpt + (int64_t)(t0 / TT) * statep + state0 : nullptr;
+    if (left > 0) {
+        request(left);
+        prepare(left);
         if (left > TT) request(left - TT);
+    }
+    for (; left > 0; left -= TT) {
+        float2 x[TT];
+#pragma unroll
+        for (int r = 0; r < TT; ++r) x[r] = row[r][lane & 15];
         if (ckpt) {
 #pragma unroll
             for (int j = 0; j < S; ++j)
                 if (q.ok && g4 * S + j < a.N) ckpt[(int64_t)j * a.D] = h[j];
             ckpt += statep;
         }
-        float2 x[TT];
-#pragma unroll
-        for (int r = 0; r < TT; ++r) x[r] = row[r][lane & 15];
+        float v[4], pz[4];
         unroll<4>([&](auto K) {
             constexpr int k = K;
             float acc[4];
             unroll<4>([&](auto I) {
                 constexpr int i = I, r = 4 * k + i;
 #pragma unroll
-                for (int j = 0; j < S; ++j) h[j] = fmaf(__builtin_amdgcn_exp2f(x[r].x * A2[j]), h[j], row_of<r>(vB.v[j]) * x[r].y);
-                if constexpr (!FIRST) acc[i] = row_dot<r>(vC.v, h);
+                for (int j = 0; j < S; ++j) h[j] = fmaf(__builtin_amdgcn_exp2f(x[r].x * A2[j]), h[j], row_of<r>(vB[j]) * x[r].y);
+                if constexpr (!FIRST) acc[i] = row_dot<r>(vC, h);
             });
             if constexpr (!FIRST) v[k] = fmaf(Dp, ku[k], swap16_add(swap32_add(acc[0], acc[2]), swap32_add(acc[1], acc[3])));
+            pz[k] = kz[k];
         });
+        // The next tile is taken over in front of this one's stores: stores and loads share a counter that is waited for in order.
+        if (left > TT) prepare(left - TT);
         if constexpr (!FIRST) {
             if (gate)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] *= kz[k] * seq_sigmoid(kz[k]);
+                for (int k = 0; k < 4; ++k) v[k] *= pz[k] * seq_sigmoid(pz[k]);
             if (q.ok) {
                 if (left >= TT) {
 #pragma unroll
@@ -309,6 +322,7 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
             }
             y += TT * a.y_st;
         }
+        if (left > 2 * TT) request(left - 2 * TT);
     }
     if constexpr (!FIRST) {
         if (q.ok)
@@ -374,241 +388,458 @@ __global__ __launch_bounds__(256) void ssm_token_kernel(SsmP p, int nvec) {
     *reinterpret_cast<Pack<E, V>*>(static_cast<E*>(a.y) + (int64_t)b * a.y_sb + d) = ry;
 }
 
-// FIRST: the launch that finds what each piece hands to the one in front of it, (a g) at its first row, from nothing behind.
-// Q passes of NW * S states each run through a tile one after another (Q > 1: more than 16 states).
-template <class E, int S, int Q, bool FIRST>
-__global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
-    constexpr int NW = 4, KT = TT / NW;
-    __shared__ float2 sd[TT][64];
-    __shared__ float sg[TT][64];
-    __shared__ float part[FIRST ? 1 : 3][FIRST ? 1 : NW][TT][64];  // of y, of sum g B, of sum (a g) h_prev A
+// Where the adjoint of a piece's last state comes from: the gradient of state_out for the last piece, otherwise what the pieces behind
+// it hand down (prod_t exp(s_t A) = exp(A sum_t s_t), as in the forward pass).
+__device__ __forceinline__ float piece_adjoint(const SsmP& p, const Place& q, int s, float A2) {
     const shivae_ssm_args& a = p.a;
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Place q = ssm_place(p, lane);
-    const int n = ssm_len(p, q.b), t0 = q.piece * p.plen, t1 = min(a.T, t0 + p.plen), tn = min(t1, n);
+    const int64_t o = ((int64_t)q.b * a.N + s) * a.D + q.d;
+    if (q.piece == p.np - 1) return a.dstate_out ? a.dstate_out[o] : 0.f;
+    float v = 0.f;
+    for (int c = p.np - 1; c > q.piece; --c)
+        v = fmaf(__builtin_amdgcn_exp2f(A2 * p.ssum[((int64_t)c * a.B + q.b) * a.D + q.d]), v, p.hend[(int64_t)c * a.B * a.N * a.D + o]);
+    return v;
+}
 
-    float ag[Q][S], A2[Q][S], dA[Q][S];
+// The operands of the backward kernels: 16-row tiles from a piece's last to its first, requested a tile ahead.
+template <class E, bool FIRST>
+struct BwdRows {
+    const E *u, *dt, *z, *dy;
+    E ru[4], rd[4], rz[4], rg[4];
+    bool gate;
+    __device__ __forceinline__ BwdRows(const shivae_ssm_args& a, const Place& q, int64_t last) {
+        u = static_cast<const E*>(a.u) + (int64_t)q.b * a.u_sb + q.d0 + last * a.u_st;
+        dt = static_cast<const E*>(a.dt) + (int64_t)q.b * a.dt_sb + q.d0 + last * a.dt_st;
+        z = static_cast<const E*>(a.z) + (int64_t)q.b * a.z_sb + q.d0 + last * a.z_st;
+        dy = static_cast<const E*>(a.dy) + (int64_t)q.b * a.dy_sb + q.d0 + last * a.dy_st;
+        gate = a.z != nullptr;
+    }
+    __device__ __forceinline__ void request(const shivae_ssm_args& a, int g4, unsigned lo, int left) {
+        const unsigned le = lo * (unsigned)sizeof(E);
+        TileRows o;
+        if (!FIRST) {
+            o.set((unsigned)a.u_st * sizeof(E), g4, le, left);
+            o.load(ru, u);
+            u -= TT * a.u_st;
+        }
+        o.set((unsigned)a.dt_st * sizeof(E), g4, le, left);
+        o.load(rd, dt);
+        dt -= TT * a.dt_st;
+        o.set((unsigned)a.dy_st * sizeof(E), g4, le, left);
+        o.load(rg, dy);
+        dy -= TT * a.dy_st;
+        if (gate) {
+            o.set((unsigned)a.z_st * sizeof(E), g4, le, left);
+            o.load(rz, z);
+            z -= TT * a.z_st;
+        }
+    }
+};
+
+// What each piece hands to the one in front of it: (a g) at its first row, from nothing behind (the last piece: from dstate_out).
+template <class E, int S>
+__global__ __launch_bounds__(256) void ssm_bwd_first_kernel(SsmP p) {
+    __shared__ float2 rows_s[4][TT][16];
+    const shivae_ssm_args& a = p.a;
+    const int lane = threadIdx.x & 63, g4 = lane >> 4;
+    float2 (&row)[TT][16] = rows_s[threadIdx.x >> 6];  // this wave's own: s, dy'
+    Place q = ssm_place(p, (int)(threadIdx.x >> 6) * 16 + (lane & 15));
+    if (!__any(q.ok)) return;
+    q.piece += 1;  // (nothing is in front of the first piece)
+    const int n = ssm_len(p, q.b), t0 = q.piece * p.plen, t1 = min(a.T, t0 + p.plen), tn = min(t1, n);
+    float ag[S], A2[S];
 #pragma unroll
-    for (int k = 0; k < Q; ++k)
+    for (int j = 0; j < S; ++j) {
+        const bool live = q.ok && g4 * S + j < a.N;
+        A2[j] = live ? a.A[(int64_t)(g4 * S + j) * a.D + q.d] * kLog2e : 0.f;
+        ag[j] = live && q.piece == p.np - 1 && a.dstate_out ? a.dstate_out[((int64_t)q.b * a.N + g4 * S + j) * a.D + q.d] : 0.f;
+    }
+    const float bias = a.dt_bias ? a.dt_bias[q.d] : 0.f;
+    const int64_t last = t0 < tn ? (tn - 1) / TT * TT : t0;
+    const E* Cm = static_cast<const E*>(a.Cm) + (int64_t)q.b * a.C_sb + (int64_t)q.g * a.C_sg + last * a.C_st;
+    const unsigned Cs = (unsigned)a.C_st * sizeof(E);
+    BwdRows<E, true> in(a, q, last);
+    RowRegs<E, S> nC;
+    float total = 0.f;
+    int left = tn - (int)last;
+    if (left > 0) {
+        in.request(a, g4, q.lo, min(left, TT));
+        nC.load(Cm, Cs, g4 * S, a.N, p.vec, left, lane);
+    }
+    for (int64_t tb = last; tb >= t0 && t0 < tn; tb -= TT, left = TT) {
+        float s[4], gy[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            s[k] = elem_f(in.rd[k]) + bias;
+            gy[k] = elem_f(in.rg[k]);
+        }
+        if (a.softplus)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] = seq_softplus(s[k]);
+        if (in.gate)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float z = elem_f(in.rz[k]);
+                gy[k] *= z * seq_sigmoid(z);
+            }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bool on = 4 * k + g4 < left;
+            s[k] = on ? s[k] : 0.f;
+            total += s[k];
+            row[4 * k + g4][lane & 15] = make_float2(s[k], on ? gy[k] : 0.f);
+        }
+        float vC[S];
+        nC.get(vC, g4 * S, a.N, left, lane);
+        if (tb > t0) {
+            in.request(a, g4, q.lo, TT);
+            Cm -= TT * a.C_st;
+            nC.load(Cm, Cs, g4 * S, a.N, p.vec, TT, lane);
+        }
+        float2 x[TT];
+#pragma unroll
+        for (int r = 0; r < TT; ++r) x[r] = row[r][lane & 15];
+        unroll<TT>([&](auto I) {
+            constexpr int r = TT - 1 - I;
+#pragma unroll
+            for (int j = 0; j < S; ++j) ag[j] = __builtin_amdgcn_exp2f(x[r].x * A2[j]) * (ag[j] + row_of<r>(vC[j]) * x[r].y);
+        });
+    }
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+        if (q.ok && g4 * S + j < a.N) p.hend[(((int64_t)q.piece * a.B + q.b) * a.N + g4 * S + j) * a.D + q.d] = ag[j];
+    total = swap32_add(total, total);
+    total = swap16_add(total, total);
+    if (q.ok && g4 == 0) p.ssum[((int64_t)q.piece * a.B + q.b) * a.D + q.d] = total;
+}
+
+// Sums over the 16 channels of a wave, for 16 rows at once.  Two rows' values are merged into one register while the lanes that still hold
+// different channels' parts halve, four times; lane l of each 16-lane row ends with row bitrev4(l)'s sum, after 33 instructions for 16
+// values.  Steps 1 and 2 (partner lane ^ 8, then mirrored in 8 lanes) write half of the banks from each of the two; steps 3 and 4 (^ 2, ^ 1)
+// need a selection.
+template <int S>
+struct Sums {
+    float b[S], c[S];
+};
+#define SV_MERGE(NAME, HOW, LO, HI)                                                                                        \
+    template <int S>                                                                                                       \
+    __device__ __forceinline__ void NAME(float (&o)[S], const float (&l)[S], const float (&h)[S]) {                        \
+        if constexpr (S == 4)                                                                                              \
+            asm("s_nop 1\n\t"                                                                                              \
+                "v_add_f32_dpp %0, %4, %4 " HOW " row_mask:0xf bank_mask:" LO "\n\t"                                       \
+                "v_add_f32_dpp %1, %5, %5 " HOW " row_mask:0xf bank_mask:" LO "\n\t"                                       \
+                "v_add_f32_dpp %2, %6, %6 " HOW " row_mask:0xf bank_mask:" LO "\n\t"                                       \
+                "v_add_f32_dpp %3, %7, %7 " HOW " row_mask:0xf bank_mask:" LO "\n\t"                                       \
+                "v_add_f32_dpp %0, %8, %8 " HOW " row_mask:0xf bank_mask:" HI "\n\t"                                       \
+                "v_add_f32_dpp %1, %9, %9 " HOW " row_mask:0xf bank_mask:" HI "\n\t"                                       \
+                "v_add_f32_dpp %2, %10, %10 " HOW " row_mask:0xf bank_mask:" HI "\n\t"                                     \
+                "v_add_f32_dpp %3, %11, %11 " HOW " row_mask:0xf bank_mask:" HI                                            \
+                : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3])                                                       \
+                : "v"(l[0]), "v"(l[1]), "v"(l[2]), "v"(l[3]), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]));                 \
+        else                                                                                                               \
+            for (int j = 0; j < S; ++j)                                                                                    \
+                asm("s_nop 1\n\t"                                                                                          \
+                    "v_add_f32_dpp %0, %1, %1 " HOW " row_mask:0xf bank_mask:" LO "\n\t"                                   \
+                    "v_add_f32_dpp %0, %2, %2 " HOW " row_mask:0xf bank_mask:" HI                                          \
+                    : "=&v"(o[j]) : "v"(l[j]), "v"(h[j]));                                                                 \
+    }
+SV_MERGE(merge8, "row_ror:8", "0x3", "0xc")
+SV_MERGE(merge4, "row_half_mirror", "0x5", "0xa")
+#undef SV_MERGE
+template <int CTRL>
+__device__ __forceinline__ float merge_quad(float lo, float hi, bool upper) {  // upper: this lane keeps hi
+    const float x = upper ? hi : lo, y = upper ? lo : hi;
+    return x + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y), CTRL, 0xf, 0xf, true));
+}
+template <int LEVEL, int S>
+__device__ __forceinline__ Sums<S> merge_rows(const Sums<S>& lo, const Sums<S>& hi, int lane) {
+    Sums<S> o;
+    if constexpr (LEVEL == 1) {
+        merge8(o.b, lo.b, hi.b);
+        merge8(o.c, lo.c, hi.c);
+    } else if constexpr (LEVEL == 2) {
+        merge4(o.b, lo.b, hi.b);
+        merge4(o.c, lo.c, hi.c);
+    } else {
+        constexpr int ctrl = LEVEL == 3 ? 0x4e : 0xb1;  // quad_perm 2 3 0 1, 1 0 3 2
+        const bool upper = lane & (LEVEL == 3 ? 2 : 1);
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const int s = (k * NW + w) * S + j;
-            const bool live = q.ok && s < a.N;
-            const int64_t o = ((int64_t)q.b * a.N + s) * a.D + q.d;
-            A2[k][j] = live ? a.A[(int64_t)s * a.D + q.d] * kLog2e : 0.f;
-            dA[k][j] = 0.f;
-            ag[k][j] = live && q.piece == p.np - 1 && a.dstate_out ? a.dstate_out[o] : 0.f;
-            if (!FIRST && live)
-                for (int c = p.np - 1; c > q.piece; --c) {
-                    const float sum = p.ssum[((int64_t)c * a.B + q.b) * a.D + q.d];
-                    ag[k][j] = fmaf(__builtin_amdgcn_exp2f(A2[k][j] * sum), ag[k][j], p.hend[(int64_t)c * a.B * a.N * a.D + o]);
-                }
+            o.b[j] = merge_quad<ctrl>(lo.b[j], hi.b[j], upper);
+            o.c[j] = merge_quad<ctrl>(lo.c[j], hi.c[j], upper);
         }
-    const float bias = a.dt_bias ? a.dt_bias[q.d] : 0.f, Dp = a.Dp ? a.Dp[q.d] : 0.f;
-    const int64_t c0 = q.d0;
-    const int last = t0 < tn ? (tn - 1) / TT * TT : t0;  // the last tile; from there to the front
-    const unsigned le = q.lo * (unsigned)sizeof(E);
-    const unsigned us = (unsigned)a.u_st * sizeof(E), ds = (unsigned)a.dt_st * sizeof(E), zs = (unsigned)a.z_st * sizeof(E), gs_ = (unsigned)a.dy_st * sizeof(E);
-    const unsigned Bs = (unsigned)a.B_st * sizeof(E), Cs = (unsigned)a.C_st * sizeof(E), os = (unsigned)((int64_t)a.B * a.D * sizeof(E));
-    const E* u = static_cast<const E*>(a.u) + (int64_t)q.b * a.u_sb + c0 + last * a.u_st;
-    const E* dt = static_cast<const E*>(a.dt) + (int64_t)q.b * a.dt_sb + c0 + last * a.dt_st;
-    const E* z = static_cast<const E*>(a.z) + (int64_t)q.b * a.z_sb + c0 + last * a.z_st;
-    const E* dy = static_cast<const E*>(a.dy) + (int64_t)q.b * a.dy_sb + c0 + last * a.dy_st;
-    const E* Bm = static_cast<const E*>(a.Bm) + (int64_t)q.b * a.B_sb + (int64_t)q.g * a.B_sg + last * a.B_st;
-    const E* Cm = static_cast<const E*>(a.Cm) + (int64_t)q.b * a.C_sb + (int64_t)q.g * a.C_sg + last * a.C_st;
-    const bool gate = a.z;
-    TileRows ou, od, oz, og, oo;
-    auto offsets = [&](int left) {
-        if (!FIRST) ou.set(us, w, le, left);
-        od.set(ds, w, le, left);
-        oz.set(zs, w, le, left);
-        og.set(gs_, w, le, left);
-    };
-    oo.set(os, w, le);
+    }
+    return o;
+}
+// f(row) for rows base + 2^LEVEL - 1 down to base, merged
+template <int LEVEL, int S, int BASE, class F>
+__device__ __forceinline__ Sums<S> sum_rows(F& f, int lane) {
+    if constexpr (LEVEL == 0) return f(std::integral_constant<int, BASE>{});
+    else {
+        const Sums<S> hi = sum_rows<LEVEL - 1, S, BASE + (1 << (LEVEL - 1))>(f, lane);
+        const Sums<S> lo = sum_rows<LEVEL - 1, S, BASE>(f, lane);
+        return merge_rows<LEVEL>(lo, hi, lane);
+    }
+}
 
-    E ru[KT], rd[KT], rz[KT], rg[KT];
-    auto request = [&]() {
-        if (!FIRST) ou.load(ru, u);
-        od.load(rd, dt);
-        if (gate) oz.load(rz, z);
-        og.load(rg, dy);
-        u -= TT * (int64_t)a.u_st;
-        dt -= TT * (int64_t)a.dt_st;
-        z -= TT * (int64_t)a.z_st;
-        dy -= TT * (int64_t)a.dy_st;
+// The backward pass of a piece.  Lanes as in the forward kernel.  A tile's rows are run forward again from the checkpoint in front of it,
+// with states and decays in registers (128 of them for S = 4), then back.  More than 16 states take several passes over a tile, 4 S
+// states each, whose adjoints and sums wait in LDS.  dB and dC are sums over all channels: of the wave's 16 by sum_rows, of the
+// workgroup's four waves through LDS (the one barrier of a pass), of the workgroups by ssm_dbc_kernel.
+template <class E, int S, bool MANY>
+__global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
+    constexpr int P = 4 * S;  // states of a pass
+    __shared__ float2 rows_s[4][TT][16];
+    __shared__ float rows_g[4][TT][16];
+    // what the end of a tile needs again, out of the way of the 8 S TT registers in between: u, dt + bias, z, dy of a lane's four rows,
+    // and the sums for y, g B and (a g) h_prev A
+    __shared__ __attribute__((aligned(16))) float4 hold_s[4][4][64];
+    __shared__ float sums_s[4][3][4][64];
+    __shared__ __attribute__((aligned(16))) float part[2][4][TT][2][P];
+    extern __shared__ __attribute__((aligned(16))) float kept[];  // [passes][3 S][256]: ag, A2, dA, where there are several passes
+    const shivae_ssm_args& a = p.a;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g4 = lane >> 4, c16 = lane & 15;
+    float2 (&row)[TT][16] = rows_s[wv];  // this wave's own: s, s u
+    float (&rowg)[TT][16] = rows_g[wv];  // dy'
+    float4 (&hold)[4][64] = hold_s[wv];
+    float (&sum3)[3][4][64] = sums_s[wv];
+    const Place q = ssm_place(p, wv * 16 + c16);
+    const int n = ssm_len(p, q.b), t0 = q.piece * p.plen, t1 = min(a.T, t0 + p.plen), tn = min(t1, n);
+    const int passes = MANY ? (a.N + P - 1) / P : 1;
+    float ag[S], A2[S], dA[S];
+    for (int k = 0; k < passes; ++k) {
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+            const int s = k * P + g4 * S + j;
+            const bool live = q.ok && s < a.N;
+            A2[j] = live ? a.A[(int64_t)s * a.D + q.d] * kLog2e : 0.f;
+            ag[j] = live ? piece_adjoint(p, q, s, A2[j]) : 0.f;
+            dA[j] = 0.f;
+            if (MANY) {
+                float* o = kept + (int64_t)k * 3 * S * 256 + threadIdx.x;
+                o[j * 256] = ag[j];
+                o[(S + j) * 256] = A2[j];
+                o[(2 * S + j) * 256] = 0.f;
+            }
+        }
+    }
+    const float bias = a.dt_bias ? a.dt_bias[q.d] : 0.f, Dp = a.Dp ? a.Dp[q.d] : 0.f;
+    const int64_t last = t0 < tn ? (tn - 1) / TT * TT : t0, statep = (int64_t)a.B * a.N * a.D;
+    const unsigned Bs = (unsigned)a.B_st * sizeof(E), Cs = (unsigned)a.C_st * sizeof(E);
+    const E* Bm = static_cast<const E*>(a.Bm) + (int64_t)q.b * a.B_sb + (int64_t)q.g * a.B_sg;
+    const E* Cm = static_cast<const E*>(a.Cm) + (int64_t)q.b * a.C_sb + (int64_t)q.g * a.C_sg;
+    BwdRows<E, false> in(a, q, last);
+
+    // B, C and the checkpoint of the next pass (of this tile or of the one in front of it)
+    RowRegs<E, S> nB, nC;
+    float nh[S];
+    auto request_states = [&](int64_t tb, int pass, int left, int lane, int g4, unsigned lo) {
+        nB.load(Bm + tb * a.B_st, Bs, pass * P + g4 * S, a.N, p.vec, left, lane);
+        nC.load(Cm + tb * a.C_st, Cs, pass * P + g4 * S, a.N, p.vec, left, lane);
+        const float* c = a.ckpt + tb / TT * statep + (int64_t)q.b * a.N * a.D + q.d0;
+#pragma unroll
+        for (int j = 0; j < S; ++j) nh[j] = at(c, (unsigned)min(pass * P + g4 * S + j, a.N - 1) * (unsigned)a.D * 4 + lo * 4);
     };
-    float total = 0.f, dDp = 0.f, dbias = 0.f;
-    int left = tn - last;
+    float dDp = 0.f, dbias = 0.f;
+    int left = tn - (int)last, buf = 0;
     if (left > 0) {
-        offsets(min(left, TT));
-        request();
-        offsets(TT);
+        in.request(a, g4, q.lo, min(left, TT));
+        request_states(last, 0, left, lane, g4, q.lo);
     }
-    for (int tb = last; tb >= t0 && t0 < tn; tb -= TT, left = TT) {
-        float ku[KT], kx[KT], kz[KT], ky[KT], ks[KT];  // u, dt + bias, z, dy, s of this thread's rows
+    for (int64_t tb = last; tb >= t0 && t0 < tn; tb -= TT, left = TT) {
+        // Opaque once a tile, so that no address that follows from them is kept in registers over the loop.
+        int lane = threadIdx.x & 63;
+        unsigned lo = q.lo;
+        asm volatile("" : "+v"(lane), "+v"(lo));
+        const int g4 = lane >> 4, c16 = lane & 15;
+        {
+            float ku[4], kx[4], kz[4] = {}, ky[4], ks[4], kg[4];
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            const int r = w + NW * k;
-            const bool in = r < left && q.ok;  // (a lane without a channel adds nothing to dB and dC)
-            ku[k] = FIRST ? 0.f : elem_f(ru[k]);
-            kx[k] = elem_f(rd[k]) + bias;
-            ks[k] = a.softplus ? seq_softplus(kx[k]) : kx[k];
-            ky[k] = elem_f(rg[k]);
-            float gy = ky[k];
-            if (gate) {
-                kz[k] = elem_f(rz[k]);
-                gy *= kz[k] * seq_sigmoid(kz[k]);
+            for (int k = 0; k < 4; ++k) {
+                ku[k] = elem_f(in.ru[k]);
+                kx[k] = ks[k] = elem_f(in.rd[k]) + bias;
+                kg[k] = ky[k] = elem_f(in.rg[k]);
             }
-            if (!in) ks[k] = 0.f;
-            sd[r][lane] = make_float2(ks[k], in ? ks[k] * ku[k] : 0.f);
-            sg[r][lane] = in ? gy : 0.f;
+            if (a.softplus)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) ks[k] = seq_softplus(kx[k]);
+            if (in.gate)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    kz[k] = elem_f(in.rz[k]);
+                    kg[k] = ky[k] * (kz[k] * seq_sigmoid(kz[k]));
+                }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool on = 4 * k + g4 < left && q.ok;  // (a lane without a channel adds nothing to dB and dC)
+                ks[k] = on ? ks[k] : 0.f;
+                row[4 * k + g4][c16] = make_float2(ks[k], on ? ks[k] * ku[k] : 0.f);
+                rowg[4 * k + g4][c16] = on ? kg[k] : 0.f;
+                hold[k][lane] = make_float4(ku[k], kx[k], kz[k], ky[k]);
+            }
         }
-        __syncthreads();
-        if (tb - TT >= t0) request();
+        if (tb > t0) in.request(a, g4, lo, TT);
+#pragma unroll 1
+        for (int pass = 0; pass < passes; ++pass) {
+            float* keep = kept + (int64_t)pass * 3 * S * 256 + threadIdx.x;
+            if (MANY)
 #pragma unroll
-        for (int k = 0; k < Q; ++k) {
-            const int s0 = (k * NW + w) * S;
-            RowRegs<E, S> vB, vC;
-            vC.load(Cm, Cs, s0, a.N, p.vec, left, lane);
-            if (!FIRST) vB.load(Bm, Bs, s0, a.N, p.vec, left, lane);
-            if constexpr (FIRST) {
-                unroll<TT>([&](auto I) {
-                    constexpr int r = TT - 1 - I;
-                    const float s = sd[r][lane].x, gy = sg[r][lane];
+                for (int j = 0; j < S; ++j) {
+                    ag[j] = keep[j * 256];
+                    A2[j] = keep[(S + j) * 256];
+                    dA[j] = keep[(2 * S + j) * 256];
+                }
+            float vB[S], vC[S], h0[S];
+            nB.get(vB, pass * P + g4 * S, a.N, left, lane);
+            nC.get(vC, pass * P + g4 * S, a.N, left, lane);
 #pragma unroll
-                    for (int j = 0; j < S; ++j) ag[k][j] = __builtin_amdgcn_exp2f(s * A2[k][j]) * fmaf(row_of<r>(vC.v[j]), gy, ag[k][j]);
-                    if (k == 0) total += s;
+            for (int j = 0; j < S; ++j) h0[j] = q.ok && pass * P + g4 * S + j < a.N ? nh[j] : 0.f;
+            if (pass + 1 < passes) request_states(tb, pass + 1, left, lane, g4, lo);
+            else if (tb > t0) request_states(tb - TT, 0, TT, lane, g4, lo);
+            float h[TT][S], e[TT][S];
+            float2 x[TT];  // read from LDS four rows ahead of their use
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = row[r][c16];
+            unroll<4>([&](auto K) {
+                constexpr int k = K;
+                float acc[4];
+                if constexpr (k < 3)
+#pragma unroll
+                    for (int i = 4; i < 8; ++i) x[4 * k + i] = row[4 * k + i][c16];
+                unroll<4>([&](auto I) {
+                    constexpr int i = I, r = 4 * k + i;
+#pragma unroll
+                    for (int j = 0; j < S; ++j) {
+                        e[r][j] = __builtin_amdgcn_exp2f(x[r].x * A2[j]);
+                        h[r][j] = fmaf(e[r][j], r ? h[r ? r - 1 : 0][j] : h0[j], row_of<r>(vB[j]) * x[r].y);
+                    }
+                    acc[i] = row_dot<r>(vC, h[r]);
                 });
-            } else {
-            // forward through the tile again: states and decays stay in registers
-            float h[TT][S], e[TT][S], first[S];
+                const float y = swap16_add(swap32_add(acc[0], acc[2]), swap32_add(acc[1], acc[3]));
+                sum3[0][k][lane] = MANY && pass ? sum3[0][k][lane] + y : y;
+                __builtin_amdgcn_sched_barrier(0);  // (or the scheduler starts all rows at once and runs out of registers)
+            });
+            // Everything that the way back takes from LDS and from B and C is taken again: kept from the way there it would be 10 S + 32
+            // registers that are not free.
+            asm volatile("" ::: "memory");
 #pragma unroll
-            for (int j = 0; j < S; ++j) {
-                first[j] = 0.f;
-                if (q.ok && s0 + j < a.N) first[j] = (a.ckpt + (((int64_t)(tb / TT) * a.B + q.b) * a.N + s0 + j) * a.D + c0)[q.lo];
+            for (int j = 0; j < S; ++j) asm volatile("" : "+v"(vB[j]), "+v"(vC[j]), "+v"(A2[j]));
+            float rb[4], rs[4], gyr[TT];
+            float2 xr[TT];
+#pragma unroll
+            for (int r = TT - 4; r < TT; ++r) {
+                xr[r] = row[r][c16];
+                gyr[r] = rowg[r][c16];
             }
-            unroll<TT>([&](auto R) {
-                constexpr int r = R;
-                const float2 s = sd[r][lane];
+            auto back = [&](auto R) {
+                constexpr int r = R, i = r & 3;
+                if constexpr (i == 3 && r > 3)
+#pragma unroll
+                    for (int t = r - 7; t < r - 3; ++t) {
+                        xr[t] = row[t][c16];
+                        gyr[t] = rowg[t][c16];
+                    }
+                const float2 x = xr[r];
+                const float gy = gyr[r];
+                Sums<S> o;
+                float g[S], gs = 0.f;
 #pragma unroll
                 for (int j = 0; j < S; ++j) {
-                    e[r][j] = __builtin_amdgcn_exp2f(s.x * A2[k][j]);
-                    h[r][j] = fmaf(e[r][j], r ? h[r ? r - 1 : 0][j] : first[j], row_of<r>(vB.v[j]) * s.y);
+                    g[j] = ag[j] + row_of<r>(vC[j]) * gy;
+                    o.c[j] = gy * h[r][j];
+                    o.b[j] = g[j] * x.y;
+                    ag[j] = e[r][j] * g[j];
+                    const float m = ag[j] * (r ? h[r ? r - 1 : 0][j] : h0[j]);
+                    gs = fmaf(m, A2[j], gs);
+                    dA[j] = fmaf(m, x.x, dA[j]);
                 }
-                const float acc = row_dot<r>(vC.v, h[r]);
-                if (gate) part[0][w][r][lane] = k ? part[0][w][r][lane] + acc : acc;
-            });
-            // and back
-            float outB = 0.f, outC = 0.f;
-            unroll<TT>([&](auto I) {
-                constexpr int r = TT - 1 - I;
-                const float2 s = sd[r][lane];
-                const float gy = sg[r][lane];
-                float g[S], gs = 0.f, xB[4] = {0.f, 0.f, 0.f, 0.f}, xC[4] = {0.f, 0.f, 0.f, 0.f};
+                rb[i] = row_dot<r>(vB, g);
+                rs[i] = gs;
+                if constexpr (i == 0) __builtin_amdgcn_sched_barrier(0);
+                if constexpr (i == 0) {
+                    const float gb = swap16_add(swap32_add(rb[0], rb[2]), swap32_add(rb[1], rb[3]));
+                    const float gs4 = swap16_add(swap32_add(rs[0], rs[2]), swap32_add(rs[1], rs[3]));
+                    sum3[1][r / 4][lane] = MANY && pass ? sum3[1][r / 4][lane] + gb : gb;
+                    sum3[2][r / 4][lane] = MANY && pass ? sum3[2][r / 4][lane] + gs4 : gs4;
+                }
+                return o;
+            };
+            const Sums<S> sums = sum_rows<4, S, 0>(back, lane);
+            const int rr = __brev((unsigned)c16) >> 28;
+            *reinterpret_cast<Pack<float, S>*>(&part[buf][wv][rr][0][g4 * S]) = *reinterpret_cast<const Pack<float, S>*>(sums.b);
+            *reinterpret_cast<Pack<float, S>*>(&part[buf][wv][rr][1][g4 * S]) = *reinterpret_cast<const Pack<float, S>*>(sums.c);
+            if (MANY)
 #pragma unroll
                 for (int j = 0; j < S; ++j) {
-                    g[j] = ag[k][j] + row_of<r>(vC.v[j]) * gy;
-                    xC[j] = gy * h[r][j];
-                    xB[j] = g[j] * s.y;
-                    ag[k][j] = e[r][j] * g[j];
-                    const float m = ag[k][j] * (r ? h[r ? r - 1 : 0][j] : first[j]);
-                    gs = fmaf(m, A2[k][j], gs);
-                    dA[k][j] = fmaf(m, s.x, dA[k][j]);
+                    keep[j * 256] = ag[j];
+                    keep[(2 * S + j) * 256] = dA[j];
                 }
-                const float gb = row_dot<r>(vB.v, g);
-                part[1][w][r][lane] = k ? part[1][w][r][lane] + gb : gb;
-                part[2][w][r][lane] = k ? part[2][w][r][lane] + gs : gs;
-                const float yB = swap16_add(swap32_add(xB[0], xB[1]), S > 2 ? swap32_add(xB[2], xB[3]) : 0.f);
-                const float yC = swap16_add(swap32_add(xC[0], xC[1]), S > 2 ? swap32_add(xC[2], xC[3]) : 0.f);
-                const float cB = row16_sum(yB), cC = row16_sum(yC);
-                if ((lane & 15) == r) {
-                    outB = cB;
-                    outC = cC;
-                }
-            });
-            const int r = lane & 15, row = lane >> 4, j = (row & 1) * 2 + (row >> 1);  // 16-lane row -> state
-            if (r < left && j < S && s0 + j < a.N) {
-                float* o = p.pbc + (((int64_t)q.tile * a.T + tb + r) * a.B + q.b) * 2 * a.N + s0 + j;
-                o[0] = outB;
-                o[a.N] = outC;
+            __syncthreads();
+            for (int i = threadIdx.x; i < TT * 2 * P; i += 256) {
+                const int r = i / (2 * P), kind = i / P & 1, s = i % P;
+                const float v = (part[buf][0][r][kind][s] + part[buf][1][r][kind][s]) + (part[buf][2][r][kind][s] + part[buf][3][r][kind][s]);
+                if (r < left && pass * P + s < a.N) p.pbc[((((int64_t)q.tile * a.T + tb + r) * a.B + q.b) * 2 + kind) * a.N + pass * P + s] = v;
             }
-            if (Q > 1) __builtin_amdgcn_sched_barrier(0);  // one pass's registers at a time
-            }
+            buf ^= 1;  // (written again behind the next barrier's far side only)
         }
-        Bm -= TT * (int64_t)a.B_st;
-        Cm -= TT * (int64_t)a.C_st;
-        __syncthreads();
-        if constexpr (!FIRST) {
+        E* const du = static_cast<E*>(a.du) + (tb * a.B + q.b) * a.D + q.d0;
+        E* const ddt = static_cast<E*>(a.ddt) + (tb * a.B + q.b) * a.D + q.d0;
+        float4 k4[4];  // u, dt + bias, z, dy
+        float ks[4], kg[4], gb[4], ds[4];
+        TileRows oo;
+        oo.set((unsigned)((int64_t)a.B * a.D * sizeof(E)), g4, lo * (unsigned)sizeof(E));
 #pragma unroll
-            for (int k = 0; k < KT; ++k) {
-                const int r = w + NW * k;
-                if (r >= left) continue;
-                float gb = 0.f, gs = 0.f;
+        for (int k = 0; k < 4; ++k) {
+            k4[k] = hold[k][lane];
+            ks[k] = row[4 * k + g4][c16].x;
+            kg[k] = rowg[4 * k + g4][c16];
+            gb[k] = sum3[1][k][lane];
+            ds[k] = fmaf(k4[k].x, gb[k], sum3[2][k][lane] * kLn2);
+        }
+        if (a.softplus)
 #pragma unroll
-                for (int i = 0; i < NW; ++i) {
-                    gb += part[1][i][r][lane];
-                    gs += part[2][i][r][lane];
-                }
-                const float gy = sg[r][lane];
-                float ds = fmaf(ku[k], gb, gs * kLn2);
-                if (a.softplus) ds *= seq_sigmoid(kx[k]);
-                const int64_t o = (int64_t)tb * a.B * a.D + (int64_t)q.b * a.D + c0;
-                if (q.ok) {
-                    put(static_cast<E*>(a.du) + o, oo.off[k], f_elem<E>(fmaf(ks[k], gb, Dp * gy)));
-                    put(static_cast<E*>(a.ddt) + o, oo.off[k], f_elem<E>(ds));
-                }
-                dbias += ds;
-                dDp = fmaf(gy, ku[k], dDp);
-                if (gate) {
-                    float y = Dp * ku[k];
+            for (int k = 0; k < 4; ++k) ds[k] *= seq_sigmoid(k4[k].y);
 #pragma unroll
-                    for (int i = 0; i < NW; ++i) y += part[0][i][r][lane];
-                    const float sig = seq_sigmoid(kz[k]);
-                    const float dz = ky[k] * y * fmaf(kz[k] * sig, 1.f - sig, sig);
-                    if (q.ok) put(static_cast<E*>(a.dz) + o, oo.off[k], f_elem<E>(dz));
-                }
+        for (int k = 0; k < 4; ++k)
+            if (4 * k + g4 < left && q.ok) {
+                put(du, oo.off[k], f_elem<E>(fmaf(ks[k], gb[k], Dp * kg[k])));
+                put(ddt, oo.off[k], f_elem<E>(ds[k]));
+                dbias += ds[k];
+                dDp = fmaf(kg[k], k4[k].x, dDp);
             }
-            __syncthreads();  // sg and part are written again by the next tile
+        if (in.gate) {
+            E* const dz = static_cast<E*>(a.dz) + (tb * a.B + q.b) * a.D + q.d0;
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float sig = seq_sigmoid(k4[k].z);
+                v[k] = k4[k].w * fmaf(Dp, k4[k].x, sum3[0][k][lane]) * fmaf(k4[k].z * sig, 1.f - sig, sig);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (4 * k + g4 < left && q.ok) put(dz, oo.off[k], f_elem<E>(v[k]));
         }
     }
-    if constexpr (FIRST) {
-        if (!q.ok) return;
-#pragma unroll
-        for (int k = 0; k < Q; ++k)
-#pragma unroll
-            for (int j = 0; j < S; ++j) {
-                const int s = (k * NW + w) * S + j;
-                if (s < a.N) p.hend[(((int64_t)q.piece * a.B + q.b) * a.N + s) * a.D + q.d] = ag[k][j];
-            }
-        if (w == 0) p.ssum[((int64_t)q.piece * a.B + q.b) * a.D + q.d] = total;
-    } else {
-    __syncthreads();
-    part[0][w][0][lane] = dDp;
-    part[0][w][1][lane] = dbias;
-    __syncthreads();
     if (!q.ok) return;
     const int64_t pb = (int64_t)q.piece * a.B + q.b;
-    if (w < 2) {
-        float v = 0.f;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) v += part[0][i][w][lane];
-        p.pD[(pb * 2 + w) * a.D + q.d] = v;
-    }
-#pragma unroll
-    for (int k = 0; k < Q; ++k)
+    dDp = swap32_add(dDp, dDp);
+    dbias = swap32_add(dbias, dbias);
+    dDp = swap16_add(dDp, dDp);
+    dbias = swap16_add(dbias, dbias);
+    if (g4 < 2) p.pD[(pb * 2 + g4) * a.D + q.d] = g4 ? dbias : dDp;
+    for (int k = 0; k < passes; ++k)
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const int s = (k * NW + w) * S + j;
+            const int s = k * P + g4 * S + j;
             if (s >= a.N) continue;
-            p.pA[(pb * a.N + s) * a.D + q.d] = dA[k][j];
-            if (q.piece == 0 && a.dstate) a.dstate[((int64_t)q.b * a.N + s) * a.D + q.d] = ag[k][j];
+            const float* keep = kept + (int64_t)k * 3 * S * 256 + threadIdx.x;
+            p.pA[(pb * a.N + s) * a.D + q.d] = MANY ? keep[(2 * S + j) * 256] : dA[j];
+            if (q.piece == 0 && a.dstate) a.dstate[((int64_t)q.b * a.N + s) * a.D + q.d] = MANY ? keep[j * 256] : ag[j];
         }
-    for (int t = max(t0, n) + w; t < t1; t += NW) {
-        const int64_t o = ((int64_t)t * a.B + q.b) * a.D + c0;
-        (static_cast<E*>(a.du) + o)[q.lo] = (E)0.f;
-        (static_cast<E*>(a.ddt) + o)[q.lo] = (E)0.f;
-        if (gate) (static_cast<E*>(a.dz) + o)[q.lo] = (E)0.f;
-    }
+    for (int t = max(t0, n) + g4; t < t1; t += 4) {
+        const int64_t o = ((int64_t)t * a.B + q.b) * a.D + q.d;
+        static_cast<E*>(a.du)[o] = (E)0.f;
+        static_cast<E*>(a.ddt)[o] = (E)0.f;
+        if (a.z) static_cast<E*>(a.dz)[o] = (E)0.f;
     }
 }
 
@@ -635,7 +866,7 @@ static int ssm_check(const shivae_ssm_args* a, const char* who) {
     SV_REQUIRE(a->N >= 1 && a->N <= 64, "%s: %d states per channel, 1..64 are supported", who, a->N);
     SV_REQUIRE(a->G >= 1 && a->D % a->G == 0, "%s: %d groups do not divide %d channels", who, a->G, a->D);
     SV_REQUIRE(a->dtype == SHIVAE_F32 || a->dtype == SHIVAE_BF16 || a->dtype == SHIVAE_F16, "%s: unknown dtype %d", who, a->dtype);
-    SV_REQUIRE(a->T <= 1 << 30 && a->D <= 1 << 24, "%s: T or D is too large", who);
+    SV_REQUIRE(a->T <= 1 << 30 && (int64_t)a->D * a->N <= 1 << 28, "%s: T or D * N is too large", who);
     SV_REQUIRE(a->u && a->dt && a->A && a->Bm && a->Cm, "%s: u, dt, A, B and C are required", who);
     // (rows of a tile are addressed by 32-bit byte offsets)
     for (int64_t st : {a->u_st, a->dt_st, a->z_st, a->y_st, a->dy_st, a->B_st, a->C_st, (int64_t)a->B * a->D})
@@ -684,18 +915,33 @@ static void launch_ssm_fwd(SsmP& p, bool first, int pieces, hipStream_t s) {
 }
 
 template <class E>
-static void launch_ssm_bwd(SsmP& p, bool first, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)p.tiles * p.a.B * p.np));
-#define SV_SSM(S, Q)                                                                                  \
-    if (first) hipLaunchKernelGGL((ssm_bwd_kernel<E, S, Q, true>), grid, dim3(256), 0, s, p);         \
-    else hipLaunchKernelGGL((ssm_bwd_kernel<E, S, Q, false>), grid, dim3(256), 0, s, p)
+static void launch_ssm_bwd_first(SsmP& p, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)p.tiles * p.a.B * (p.np - 1)));
+#define SV_SSM(S) hipLaunchKernelGGL((ssm_bwd_first_kernel<E, S>), grid, dim3(256), 0, s, p)
     const int N = p.a.N;
-    ssm_vec(p, N <= 8 ? 2 : 4);
-    if (N <= 8) { SV_SSM(2, 1); }
-    else if (N <= 16) { SV_SSM(4, 1); }
-    else if (N <= 32) { SV_SSM(4, 2); }
-    else { SV_SSM(4, 4); }
+    ssm_vec(p, N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16);
+    if (N <= 4) SV_SSM(1);
+    else if (N <= 8) SV_SSM(2);
+    else if (N <= 16) SV_SSM(4);
+    else if (N <= 32) SV_SSM(8);
+    else SV_SSM(16);
 #undef SV_SSM
+}
+
+template <class E>
+static int launch_ssm_bwd(SsmP& p, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)p.tiles * p.a.B * p.np));
+    const int N = p.a.N, S = N <= 4 ? 1 : N <= 8 ? 2 : 4, passes = ceil_div(N, 4 * S);
+    const size_t lds = passes > 1 ? (size_t)passes * 3 * S * 256 * sizeof(float) : 0;  // up to 48 KiB beside 28 of static
+    ssm_vec(p, S);
+    if (lds)  // (past the default limit of 64 KiB)
+        SV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_bwd_kernel<E, 4, true>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (S == 1) hipLaunchKernelGGL((ssm_bwd_kernel<E, 1, false>), grid, dim3(256), 0, s, p);
+    else if (S == 2) hipLaunchKernelGGL((ssm_bwd_kernel<E, 2, false>), grid, dim3(256), 0, s, p);
+    else if (passes == 1) hipLaunchKernelGGL((ssm_bwd_kernel<E, 4, false>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((ssm_bwd_kernel<E, 4, true>), grid, dim3(256), lds, s, p);
+    SV_CHECK_HIP(hipGetLastError());
+    return SHIVAE_OK;
 }
 
 }  // namespace shivae
@@ -772,8 +1018,8 @@ int shivae_selective_scan_bwd(const shivae_ssm_args* args, void* ws_dev, size_t 
     p.pbc = p.hend + piece_floats(p);
     p.pA = p.pbc + (size_t)p.tiles * a.T * a.B * 2 * a.N;
     p.pD = p.pA + (size_t)p.np * a.B * a.N * a.D;
-    if (p.np > 1) SV_BY_DTYPE(a.dtype, launch_ssm_bwd<E>(p, true, s));
-    SV_BY_DTYPE(a.dtype, launch_ssm_bwd<E>(p, false, s));
+    if (p.np > 1) SV_BY_DTYPE(a.dtype, launch_ssm_bwd_first<E>(p, s));
+    SV_BY_DTYPE(a.dtype, SV_TRY(launch_ssm_bwd<E>(p, s)));
     SV_CHECK_HIP(hipGetLastError());
     const int64_t total = (int64_t)a.T * a.B * a.G * 2 * a.N;
     const dim3 grid((unsigned)((total + 255) / 256));
