@@ -5,7 +5,7 @@
 //   token = the first index i, in index order, with  sum_{kept j <= i} w_j > u * sum_{kept j} w_j
 //
 // Which category is drawn hangs on comparisons of long sums, and 16-bit logits have long runs of equal values, whose errors add up
-// in step.  So a weight is computed in 64 bits (a polynomial for 2^f, error below 2^-47) and held as a multiple of 2^-43 of the
+// in step.  So a weight is computed in 64 bits (a polynomial for 2^f, error below 2^-36) and held as a multiple of 2^-43 of the
 // largest: sums of these are exact, independent of order (integer LDS atomics included), and fit 63 bits for 2^20 categories.  A
 // weight below 2^-44 of the largest is 0 and is never drawn.  Order is by the logits' own bits, never by rounded quotients.
 //
@@ -42,7 +42,7 @@ __device__ __forceinline__ RowParams row_params(const shivae_sample_args& a, int
 }
 
 // A logit as it is compared: NaN counts as -inf, -0 as 0.
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.f; }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY) + 0.f; }
 // Unsigned keys in the order of the values, and back.
 __device__ __forceinline__ unsigned key_of(float x) {
     const unsigned b = __float_as_uint(x);
@@ -51,12 +51,13 @@ __device__ __forceinline__ unsigned key_of(float x) {
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
 constexpr int kFix = 43;
-// 2^y for y <= 0: 2^f = sum (f ln 2)^k / k!, |f| <= 1/2; the first dropped term is (0.3466)^12 / 12! = 6e-15.
+// 2^(y + shift) for -900 <= y <= 0: 2^f = sum (f ln 2)^k / k!, |f| <= 1/2; the first dropped term is (0.3466)^10 / 10! = 7e-12 = 2^-37.
+// Adding 1.5 2^52 rounds y to a whole number and leaves it in the low word; the exponent is added to the high word (v_rndne_f64,
+// v_ldexp_f64 and the conversion cost several fused operations each).
 __device__ __forceinline__ double exp2_f64(double y, int shift) {
-    const double n = rint(y), f = y - n;
-    double p = 4.4455382718708115e-10;
-    p = fma(p, f, 7.0549116208011234e-09);
-    p = fma(p, f, 1.0178086009239699e-07);
+    constexpr double magic = 6755399441055744.0;
+    const double t = y + magic, f = y - (t - magic);
+    double p = 1.0178086009239699e-07;
     p = fma(p, f, 1.3215486790144309e-06);
     p = fma(p, f, 1.5252733804059841e-05);
     p = fma(p, f, 1.5403530393381608e-04);
@@ -66,7 +67,9 @@ __device__ __forceinline__ double exp2_f64(double y, int shift) {
     p = fma(p, f, 2.4022650695910072e-01);
     p = fma(p, f, 6.9314718055994531e-01);
     p = fma(p, f, 1.0);
-    return ldexp(p, (int)n + shift);
+    const u64 b = (u64)__double_as_longlong(p);
+    const unsigned hi = (unsigned)(b >> 32) + (((unsigned)__double_as_longlong(t) + (unsigned)shift) << 20);
+    return __longlong_as_double((long long)((u64)hi << 32 | (unsigned)b));
 }
 // The weight of x as a multiple of 2^-43: adding 2^52 rounds to whole numbers and leaves them in the mantissa.
 struct Weigh {
@@ -79,19 +82,30 @@ struct Weigh {
         least = min_p > 0.f ? fmax(log2((double)min_p), -44.0) : -44.0;
     }
     __device__ __forceinline__ bool enough(float x) const { return log2w(x) >= least; }  // min-p
+    // No branch: eight elements' chains of dependent operations run side by side.  -inf (and -inf * 0) become 2^-200, which rounds to 0.
     __device__ __forceinline__ u64 fix(float x) const {
-        const double y = log2w(x);
-        if (!(y >= -44.0)) return 0;
-        return (u64)__double_as_longlong(exp2_f64(y, kFix) + 4503599627370496.0) & 0xfffffffffffffull;
+        return (u64)__double_as_longlong(exp2_f64(fmax(log2w(x), -200.0), kFix) + 4503599627370496.0) & 0xfffffffffffffull;
     }
 };
 
 __device__ __forceinline__ u64 shfl_u64(u64 v, int lane) { return (u64)__shfl((long long)v, lane, 64); }
 __device__ __forceinline__ u64 shfl_up_u64(u64 v, int d) { return (u64)__shfl_up((long long)v, d, 64); }
+// The sum over the wave's lanes, in every lane: rotations within rows of 16 lanes, then exchanges of rows (no LDS round trips).
+template <int CTRL>
+__device__ __forceinline__ u64 ror_add(u64 v) {
+    const unsigned lo = __builtin_amdgcn_mov_dpp((unsigned)v, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp((unsigned)(v >> 32), CTRL, 0xf, 0xf, true);
+    return v + ((u64)hi << 32 | lo);
+}
 __device__ __forceinline__ u64 wave_sum(u64 v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += (u64)__shfl_xor((long long)v, d, 64);
-    return v;
+    v = ror_add<0x128>(v);
+    v = ror_add<0x124>(v);
+    v = ror_add<0x122>(v);
+    v = ror_add<0x121>(v);
+    auto l = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false), h = __builtin_amdgcn_permlane16_swap((unsigned)(v >> 32), (unsigned)(v >> 32), false, false);
+    v = ((u64)h[0] << 32 | l[0]) + ((u64)h[1] << 32 | l[1]);
+    l = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+    h = __builtin_amdgcn_permlane32_swap((unsigned)(v >> 32), (unsigned)(v >> 32), false, false);
+    return ((u64)h[0] << 32 | l[0]) + ((u64)h[1] << 32 | l[1]);
 }
 
 // ------------------------------------------------------------------------------------------------ a workgroup per row
@@ -132,6 +146,38 @@ struct Sampler {
         if (has_inf)
 #pragma unroll
             for (int k = 0; k < VE; ++k) x[k] = x[k] == INFINITY ? 0.f : -INFINITY;
+    }
+
+    // f(i, x) for every vector of the row, by whole waves of 64 neighbouring vectors (the last wave's lanes behind the row hold -inf).  Four
+    // loads of a thread are in flight at a time: with one, each pass waits 16 times for L2 at 131072 categories.
+    template <class F>
+    __device__ __forceinline__ void sweep(F f) const {
+        constexpr int U = 4;
+        const int end = (nvec + 63) & ~63;
+        for (int i0 = tid; i0 < end; i0 += U * NT) {
+            Pack<E, VE> raw[U];
+#pragma unroll
+            for (int t = 0; t < U; ++t) {
+                const int j0 = (i0 + t * NT) * VE - off;
+                if (j0 >= 0 && j0 + VE <= V) raw[t] = *reinterpret_cast<const Pack<E, VE>*>(p + j0);
+            }
+#pragma unroll
+            for (int t = 0; t < U; ++t) {
+                const int i = i0 + t * NT, j0 = i * VE - off;
+                if (i >= end) break;
+                float x[VE];
+                if (j0 >= 0 && j0 + VE <= V) {
+#pragma unroll
+                    for (int k = 0; k < VE; ++k) x[k] = clean(elem_f(raw[t].v[k]));
+                    if (has_inf)
+#pragma unroll
+                        for (int k = 0; k < VE; ++k) x[k] = x[k] == INFINITY ? 0.f : -INFINITY;
+                } else {
+                    get(i, x);
+                }
+                f(i, x);
+            }
+        }
     }
 
     // Exclusive sum of v over the workgroup's threads, and the whole sum.  Ends with a barrier behind the last read.
@@ -190,8 +236,32 @@ struct Sampler {
         return at;
     }
 
-    // list[0, n), padded to a power of two with zeros, into descending order.
+    // list[0, n) into descending order (entries differ, but for zeros, which end up behind the rest).  Short lists by counting what is
+    // larger, at two barriers; longer ones, padded to a power of two with zeros, by a bitonic network, a barrier for each of its steps.
     __device__ __forceinline__ void sort(int n) {
+        constexpr int R = 1024 / NT > 1 ? 2 : 1;  // elements per thread
+        if (n <= R * NT && n <= 1024) {
+            u64 e[R];
+            int rank[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int i = tid + r * NT;
+                e[r] = i < n ? s.list[i] : 0;
+                rank[r] = 0;
+            }
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) {
+                const u64 o = s.list[j];
+#pragma unroll
+                for (int r = 0; r < R; ++r) rank[r] += o > e[r] || (o == e[r] && j < tid + r * NT);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (tid + r * NT < n) s.list[rank[r]] = e[r];
+            __syncthreads();
+            return;
+        }
         int m = 1;
         while (m < n) m <<= 1;
         for (int i = n + tid; i < m; i += NT) s.list[i] = 0;
@@ -215,30 +285,31 @@ struct Sampler {
     template <class B, class W>
     __device__ __forceinline__ void fill(int bins, B bin_of, W value) {
         clear(bins);
-        for (int i = tid; i < ((nvec + 63) & ~63); i += NT) {  // whole waves, for the ballot
-            float x[VE];
+        sweep([&](int i, const float (&x)[VE]) {
             int b[VE];
-            if (i < nvec) get(i, x);
             bool same = true;
 #pragma unroll
             for (int k = 0; k < VE; ++k) {
-                b[k] = i < nvec ? bin_of(x[k], i * VE + k - off) : -1;
+                b[k] = bin_of(x[k], i * VE + k - off);
                 same &= b[k] == b[0];
             }
             const int first = __builtin_amdgcn_readfirstlane(b[0]);
             if (__ballot(same && b[0] == first) == ~0ull) {
-                if (first < 0) continue;
+                if (first < 0) return;
                 u64 v = 0;
 #pragma unroll
                 for (int k = 0; k < VE; ++k) v += value(x[k]);
                 v = wave_sum(v);
                 if (lane == 0) atomicAdd(&s.hist[first], v);
             } else {
+                u64 v[VE];
+#pragma unroll
+                for (int k = 0; k < VE; ++k) v[k] = value(x[k]);
 #pragma unroll
                 for (int k = 0; k < VE; ++k)
-                    if (b[k] >= 0) atomicAdd(&s.hist[b[k]], value(x[k]));
+                    if (b[k] >= 0) atomicAdd(&s.hist[b[k]], v[k]);
             }
-        }
+        });
         __syncthreads();
     }
     // Puts the elements that take(x, index) holds into the list, in any order, as far as there is room; -> their number.
@@ -246,18 +317,16 @@ struct Sampler {
     __device__ __forceinline__ int gather(F take) {
         if (tid == 0) s.count = 0;
         __syncthreads();
-        for (int i = tid; i < nvec; i += NT) {
-            float x[VE];
-            get(i, x);
+        sweep([&](int i, const float (&x)[VE]) {
             unsigned m = 0;
 #pragma unroll
             for (int k = 0; k < VE; ++k) m |= take(x[k], i * VE + k - off) ? 1u << k : 0u;
-            if (!m) continue;
+            if (!m) return;
             int at = atomicAdd(&s.count, __popc(m));
 #pragma unroll
             for (int k = 0; k < VE; ++k)
                 if ((m >> k & 1) && at < CAP) s.list[at++] = place(x[k], i * VE + k - off);
-        }
+        });
         __syncthreads();
         const int n = s.count;
         __syncthreads();
@@ -274,7 +343,7 @@ struct Sampler {
 
     // (max - x) scaled to bins: monotone in x, so bins are in the order of the values.  NB - 1: no weight.
     float top, bscale;
-    __device__ __forceinline__ int bin(float x) const { return x == -INFINITY ? NB - 1 : (int)fminf((top - x) * bscale, (float)(NB - 1)); }
+    __device__ __forceinline__ int bin(float x) const { return (int)fminf((top - x) * bscale, (float)(NB - 1)); }  // (-inf, NaN: the last)
 
     __device__ __forceinline__ int has_weight(float x) const {  // its bin, or -1
         const int b = bin(x);
@@ -310,26 +379,51 @@ struct Sampler {
         const u64 w = weight(x0), nth = w ? (g - before) / w : 0;
         u64 bf, total;
         float xv;
-        const int idx = locate([&](float x, int i) { return (u64)(x == x0 && place(x, i) >= last); }, [&](u64) { return nth; }, bf, total, xv);
+        const int idx = locate([&](float x, int i) { return x == x0 && place(x, i) >= last; }, [](float) { return (u64)1; }, [&](u64) { return nth; }, bf, total, xv);
         return place(x0, idx < 0 ? V - 1 : idx);
     }
 
-    // The first index, in index order, at which the running sum of weight(x, index) exceeds goal(total); -1 if none.  Sums of
-    // 64-vector segments first, then one wave looks into the segment.
-    template <class W, class G>
-    __device__ __forceinline__ int locate(W weight, G goal, u64& before, u64& total, float& value) {
+    // The first index, in index order, at which the running sum of weight(x), over what take(x, index) holds of, exceeds goal(total); -1
+    // if none.  Sums of 64-vector segments first, then one wave looks into the segment.  A wave whose segment is at most half taken
+    // first puts those elements side by side (in its part of the list), so that weights are computed for full waves of them.
+    template <class T, class W, class G>
+    __device__ __forceinline__ int locate(T take, W weight, G goal, u64& before, u64& total, float& value) {
         const int nseg = (nvec + 63) / 64;
-        for (int i = tid; i < nseg * 64; i += NT) {
-            float x[VE];
-            u64 sum = 0;
-            if (i < nvec) {
-                get(i, x);
+        constexpr int PER = 64 * VE;  // elements of a segment
+        float* mine = reinterpret_cast<float*>(s.list) + wv * PER;
+        constexpr bool room = (size_t)NWV * PER * sizeof(float) <= sizeof(s.list);
+        sweep([&](int i, const float (&x)[VE]) {
+            bool in[VE];
+            int all = 0;  // elements taken by the wave
 #pragma unroll
-                for (int k = 0; k < VE; ++k) sum += weight(x[k], i * VE + k - off);
+            for (int k = 0; k < VE; ++k) {
+                in[k] = take(x[k], i * VE + k - off);
+                all += __popcll(__ballot(in[k]));
             }
-            sum = wave_sum(sum);
+            u64 sum = 0;
+            if (room && all <= PER / 2) {
+                int at = 0;
+#pragma unroll
+                for (int k = 0; k < VE; ++k) {
+                    const u64 on = __ballot(in[k]);
+                    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(on >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)on, 0));
+                    if (in[k]) mine[at + before] = x[k];
+                    at += __popcll(on);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 4
+                for (int j = lane; j < all; j += 64) sum += weight(mine[j]);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            } else {
+                u64 w[VE];
+#pragma unroll
+                for (int k = 0; k < VE; ++k) w[k] = weight(x[k]);
+#pragma unroll
+                for (int k = 0; k < VE; ++k) sum += in[k] ? w[k] : 0;
+            }
+            if (all) sum = wave_sum(sum);
             if (lane == 0) s.hist[i >> 6] = sum;
-        }
+        });
         __syncthreads();
         u64 g = 0;
         const int seg = first_beyond(nseg, [&](int i) { return s.hist[i]; }, [&](u64 t) { return g = goal(t); }, before, total);
@@ -342,7 +436,7 @@ struct Sampler {
             if (i < nvec) get(i, x);
 #pragma unroll
             for (int k = 0; k < VE; ++k) {
-                w[k] = i < nvec ? weight(x[k], i * VE + k - off) : 0;
+                w[k] = i < nvec && take(x[k], i * VE + k - off) ? weight(x[k]) : 0;
                 sum += w[k];
             }
             u64 in = sum;
@@ -372,35 +466,46 @@ struct Sampler {
         return idx;
     }
 
-    __device__ __forceinline__ void run(const RowParams& q, int64_t* token, float* logprob) {
-        // 1. the largest, lowest index first
-        u64 best = 0;
-        for (int i = tid; i < nvec; i += NT) {
+    __device__ __forceinline__ float block_max(float v) {
+#pragma unroll
+        for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+        if (NWV > 1) {
+            if (lane == 0) s.wave[wv] = __float_as_uint(v);
+            __syncthreads();
+            for (int i = 0; i < NWV; ++i) v = fmaxf(v, __uint_as_float((unsigned)s.wave[i]));
+            __syncthreads();
+        }
+        return v;
+    }
+    // The lowest index at which the row holds x.
+    __device__ __forceinline__ int first_equal(float x0) {
+        if (tid == 0) s.pos = V;
+        __syncthreads();
+        int at = V;
+        for (int i = tid; i < nvec && at == V; i += NT) {
             float x[VE];
             get(i, x);
 #pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                const int idx = i * VE + k - off;
-                const u64 e = place(x[k], idx);
-                if (idx >= 0 && idx < V && e > best) best = e;
-            }
+            for (int k = VE - 1; k >= 0; --k)
+                if (x[k] == x0) at = i * VE + k - off;
         }
+        if (at < V) atomicMin(&s.pos, at);
+        __syncthreads();
+        return s.pos;
+    }
+
+    __device__ __forceinline__ void run(const RowParams& q, int64_t* token, float* logprob) {
+        // 1. the largest
+        float most = -INFINITY;
+        sweep([&](int, const float (&x)[VE]) {
 #pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            const u64 o = (u64)__shfl_xor((long long)best, d, 64);
-            best = o > best ? o : best;
-        }
-        if (NWV > 1) {
-            if (lane == 0) s.wave[wv] = best;
-            __syncthreads();
-            for (int i = 0; i < NWV; ++i) best = s.wave[i] > best ? s.wave[i] : best;
-            __syncthreads();
-        }
-        top = of_key((unsigned)(best >> 32));
-        const int arg = (int)(0xffffffffu - (unsigned)best);
+            for (int k = 0; k < VE; ++k) most = fmaxf(most, x[k]);
+        });
+        top = block_max(most);
         if (top == -INFINITY || !(q.temperature > 0.f)) {
+            const int arg = top == -INFINITY ? -1 : first_equal(top);
             if (tid == 0) {
-                *token = top == -INFINITY ? -1 : arg;
+                *token = arg;
                 if (logprob) *logprob = top == -INFINITY ? -INFINITY : 0.f;
             }
             return;
@@ -465,14 +570,12 @@ struct Sampler {
             // 4. the draw over the row
             const float low = of_key((unsigned)(last >> 32));
             const bool all = last == 0;
+            const float least = smallest(wt);
             idx = locate(
-                [&](float x, int i) {
-                    if (!all && (x < low || (x == low && place(x, i) < last))) return (u64)0;
-                    return wt.enough(x) ? wt.fix(x) : 0;
-                },
+                [&](float x, int i) { return (all || x > low || (x == low && place(x, i) >= last)) && x >= least; }, fix,
                 [&](u64 t) { return draw(q.u, t); }, before, total, xv);
-            if (idx < 0) {
-                idx = arg;
+            if (idx < 0) {  // (not reached: the largest is always kept)
+                idx = first_equal(top);
                 xv = top;
             }
         }
@@ -480,6 +583,17 @@ struct Sampler {
             *token = idx;
             if (logprob) *logprob = (float)(wt.log2w(xv) * 0.69314718055994530942 - log(ldexp((double)total, -kFix)));
         }
+    }
+    // The smallest value with w >= min_p and a weight at all: between two values a step apart there is none, so comparing values is
+    // comparing weights.
+    __device__ __forceinline__ float smallest(const Weigh& wt) const {
+        unsigned lo = key_of(-INFINITY) + 1, hi = key_of(top);  // the least key for which enough() holds is in [lo, hi]
+        while (lo < hi) {
+            const unsigned mid = lo + (hi - lo) / 2;
+            if (wt.enough(of_key(mid))) hi = mid;
+            else lo = mid + 1;
+        }
+        return of_key(lo);
     }
     // Running sums are whole numbers: sum >= p * total is sum > ceil(p * total) - 1, sum > u * total is sum > floor(u * total).
     __device__ static u64 lead(float p, u64 total) {
