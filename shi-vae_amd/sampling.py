@@ -12,11 +12,11 @@ MAX_CATEGORIES = 1048512  # SHIVAE_SAMPLE_MAX
 
 def _setting(v, name, shape, device, dtype, low, high=None):
     """A number for all rows, or a tensor with one for each -> (pointer owner, number)."""
-    if torch.is_tensor(v):
+    if isinstance(v, torch.Tensor):
         if v.device != device:
             raise ValueError("%s is on %s, not on %s" % (name, v.device, device))
-        if tuple(v.shape) != shape:
-            raise ValueError("%s has shape %s, expected a number or %s" % (name, tuple(v.shape), shape))
+        if v.shape != shape:
+            raise ValueError("%s has shape %s, expected a number or %s" % (name, tuple(v.shape), tuple(shape)))
         if v.is_floating_point() != dtype.is_floating_point or v.dtype == torch.bool:
             raise TypeError("%s is %s, expected %s" % (name, v.dtype, dtype))
         if v.dtype == torch.int64:
@@ -41,7 +41,7 @@ def sample_categories(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
 
     Returns int64 indices [...], or (indices, log-probability of the index among the kept [...] float32); the log-probability
     is 0 for temperature 0 and -inf where the index is -1."""
-    if not torch.is_tensor(logits) or logits.dtype not in _DTYPES:
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES:
         raise TypeError("logits must be a float32, bfloat16 or float16 tensor")
     if logits.dim() < 1 or logits.numel() == 0:
         raise ValueError("logits of shape %s have nothing to draw from" % (tuple(logits.shape),))
@@ -50,16 +50,16 @@ def sample_categories(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
         raise ValueError("%d categories, up to %d are supported" % (V, MAX_CATEGORIES))
     if not logits.is_cuda:
         raise N.ShiVAENativeError("sample_categories runs as a HIP kernel: the logits are on %s and there is no CPU fallback" % logits.device)
-    dev, shape = logits.device, tuple(logits.shape[:-1])
-    if not torch.is_tensor(u) or u.dtype != torch.float32:
+    dev, shape = logits.device, logits.shape[:-1]
+    if not isinstance(u, torch.Tensor) or u.dtype is not torch.float32:
         raise TypeError("u must be a float32 tensor")
-    if u.device != dev or tuple(u.shape) != shape:
-        raise ValueError("u must have shape %s and lie on %s" % (shape, dev))
+    if u.shape != shape or u.device != dev:
+        raise ValueError("u must have shape %s and lie on %s" % (tuple(shape), dev))
     t_rows, t = _setting(temperature, "temperature", shape, dev, torch.float32, 0.0)
     k_rows, k = _setting(top_k, "top_k", shape, dev, torch.int32, 0)
     p_rows, p = _setting(top_p, "top_p", shape, dev, torch.float32, 0.0, 1.0)
     m_rows, m = _setting(min_p, "min_p", shape, dev, torch.float32, 0.0, 1.0)
-    rows = logits.detach().reshape(-1, V)
+    rows = logits.detach().reshape(-1, V) if logits.dim() != 2 else logits
     if rows.stride(1) != 1 and V > 1:
         rows = rows.contiguous()
     u = u.contiguous()
