@@ -161,14 +161,14 @@ struct Sampler {
                 const int j0 = (i0 + t * NT) * VE - off;
                 if (j0 >= 0 && j0 + VE <= V) raw[t] = *reinterpret_cast<const Pack<E, VE>*>(p + j0);
             }
-#pragma unroll
-            for (int t = 0; t < U; ++t) {
-                const int i = i0 + t * NT, j0 = i * VE - off;
-                if (i >= end) break;
+            // (one copy of f: unrolled four times the passes of a row do not fit the instruction cache)
+#pragma unroll 1
+            for (int i = i0; i < min(end, i0 + U * NT); i += NT) {
+                const int j0 = i * VE - off;
                 float x[VE];
                 if (j0 >= 0 && j0 + VE <= V) {
 #pragma unroll
-                    for (int k = 0; k < VE; ++k) x[k] = clean(elem_f(raw[t].v[k]));
+                    for (int k = 0; k < VE; ++k) x[k] = clean(elem_f(raw[0].v[k]));
                     if (has_inf)
 #pragma unroll
                         for (int k = 0; k < VE; ++k) x[k] = x[k] == INFINITY ? 0.f : -INFINITY;
@@ -176,6 +176,8 @@ struct Sampler {
                     get(i, x);
                 }
                 f(i, x);
+#pragma unroll
+                for (int t = 0; t + 1 < U; ++t) raw[t] = raw[t + 1];
             }
         }
     }

@@ -3,19 +3,19 @@
 // Backward, with g[n] = dL/dh[n] running from the last row to the first and dy' = dy silu(z):
 //   g[n] = C[n] dy' + (a g)[n] of the next row;  dC[n] = sum_d dy' h[n];  dB[n] = sum_d g[n] s u
 //   ds = sum_n (a g)[n] h_prev[n] A[n] + u sum_n g[n] B[n];  du = s sum_n g[n] B[n] + Dp dy';  dA[n] = sum_t (a g)[n] h_prev[n] s
-// A is general (one number per channel and state), so the recurrence is element-wise in (d, n) and has no matrix form:
-// one exponential, one product and two fused multiply-adds per (row, channel, state).  A wave64 instruction takes 4 cycles,
-// the exponential 16, so 16 states cost 512 cycles per row and 64 channels, softplus and the gate about 160 more: the
-// whole card does 235 G (row, channel) pairs a second, which is 1.9 TB/s of bf16 traffic.  Bound by vector instructions,
-// not by memory.
+// A is general (one number per channel and state), so the recurrence is element-wise in (d, n) and has no matrix form: one exponential,
+// two products and two fused multiply-adds per (row, channel, state).  Measured here a vector instruction of a wave takes 4 cycles, an
+// exponential 8, so the forward pass of 16 states is 16 * 24 = 384 cycles per row and 64 channels, softplus and the gate about 100 more:
+// at most 325 G (row, channel) pairs a second on the whole card, 2.6 TB/s of bf16 traffic.  Bound by vector instructions, not by memory.
 //
-// Layout: lane = channel (64 neighbouring channels per workgroup, one cache line of bf16), the states of a channel are dealt
-// to the workgroup's waves, S to each.  Rows come in tiles of 16: all threads together load u, dt, z, B, C of the next tile
-// while the present one runs, and put s and s u (once per channel, not once per wave) and fp32 copies of B and C into LDS;
-// every wave then runs its states through the tile and leaves its part of y in LDS; all threads add the parts, gate, store.
-// Where B * D is small, the time axis is split into pieces: a first launch runs each piece from a zero state and keeps its
-// last state and sum of s; since prod_t exp(s_t A) = exp(A sum_t s_t), a piece of the second launch gets its first state
-// from those of the pieces in front of it.
+// Layout: lane = (state group, channel): a wave owns 16 neighbouring channels and all their states, a workgroup 64 channels of a sequence
+// (one cache line of bf16).  Rows come in tiles of 16, requested a tile ahead.  Where B * D is small the time axis is split into pieces: a
+// first launch runs each piece from a zero state and keeps its last state and sum of s; since prod_t exp(s_t A) = exp(A sum_t s_t), a piece
+// of the second launch gets its first state from those of the pieces in front of it (backward: the adjoint from those behind).
+// Measured (MI355X, us): T 2048, B 16, D 2048, N 16, bf16, gate: 350 (1.55 TB/s); at B 64 1095, 245 G pairs a second, 0.75 of the bound: at
+// B 16 a SIMD has two waves, whose dependent exponentials are not covered.  T 8192, B 1: 150 in 32 pieces; in 16 pieces 167.
+// Earlier forms of the same kernel, at B 16: 64 channels a wave and the states over four waves, s, B and C from LDS: 404 (64 of its 96 LDS
+// cycles per row were broadcasts of B and C); B and C by scalar loads: 757; by row_newbcast: 415; waves that share nothing: 350.
 #include <algorithm>
 #include <utility>
 
@@ -44,6 +44,9 @@ __device__ __forceinline__ int ssm_len(const SsmP& p, int b) {
     const int n = p.a.lengths[b];
     return n < 0 ? 0 : (n < p.a.T ? n : p.a.T);
 }
+
+// A log2(e), finite: an A of -inf (no memory) has to give exp(0 A) = 1 behind a sequence's end, and 0 where a step is positive.
+__device__ __forceinline__ float scale_A(float A) { return fminf(fmaxf(A * kLog2e, -3.4e38f), 3.4e38f); }
 
 // One workgroup's place: piece, sequence, group, and this lane's channel.
 struct Place {
@@ -204,7 +207,7 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
     for (int j = 0; j < S; ++j) {
         const bool live = q.ok && g4 * S + j < a.N;
         const int64_t o = state0 + (int64_t)j * a.D;
-        A2[j] = live ? a.A[(int64_t)(g4 * S + j) * a.D + q.d] * kLog2e : 0.f;
+        A2[j] = live ? scale_A(a.A[(int64_t)(g4 * S + j) * a.D + q.d]) : 0.f;
         h[j] = live && q.piece == 0 && a.state ? a.state[o] : 0.f;
         if (!FIRST && live)
             for (int c = 0; c < q.piece; ++c) {
@@ -373,7 +376,7 @@ __global__ __launch_bounds__(256) void ssm_token_kernel(SsmP p, int nvec) {
             const float Bn = elem_f(Bm[n]), Cn = elem_f(Cm[n]);
 #pragma unroll
             for (int c = 0; c < V; ++c) {
-                h.v[c] = fmaf(__builtin_amdgcn_exp2f(s[c] * (A.v[c] * kLog2e)), h.v[c], s[c] * u[c] * Bn);
+                h.v[c] = fmaf(__builtin_amdgcn_exp2f(s[c] * scale_A(A.v[c])), h.v[c], s[c] * u[c] * Bn);
                 y[c] = fmaf(Cn, h.v[c], y[c]);
             }
         }
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(256) void ssm_bwd_first_kernel(SsmP p) {
 #pragma unroll
     for (int j = 0; j < S; ++j) {
         const bool live = q.ok && g4 * S + j < a.N;
-        A2[j] = live ? a.A[(int64_t)(g4 * S + j) * a.D + q.d] * kLog2e : 0.f;
+        A2[j] = live ? scale_A(a.A[(int64_t)(g4 * S + j) * a.D + q.d]) : 0.f;
         ag[j] = live && q.piece == p.np - 1 && a.dstate_out ? a.dstate_out[((int64_t)q.b * a.N + g4 * S + j) * a.D + q.d] : 0.f;
     }
     const float bias = a.dt_bias ? a.dt_bias[q.d] : 0.f;
@@ -611,7 +614,7 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
         for (int j = 0; j < S; ++j) {
             const int s = k * P + g4 * S + j;
             const bool live = q.ok && s < a.N;
-            A2[j] = live ? a.A[(int64_t)s * a.D + q.d] * kLog2e : 0.f;
+            A2[j] = live ? scale_A(a.A[(int64_t)s * a.D + q.d]) : 0.f;
             ag[j] = live ? piece_adjoint(p, q, s, A2[j]) : 0.f;
             dA[j] = 0.f;
             if (MANY) {
@@ -870,7 +873,7 @@ static int ssm_check(const shivae_ssm_args* a, const char* who) {
     SV_REQUIRE(a->u && a->dt && a->A && a->Bm && a->Cm, "%s: u, dt, A, B and C are required", who);
     // (rows of a tile are addressed by 32-bit byte offsets)
     for (int64_t st : {a->u_st, a->dt_st, a->z_st, a->y_st, a->dy_st, a->B_st, a->C_st, (int64_t)a->B * a->D})
-        SV_REQUIRE(st >= 0 && st * elem_bytes(a->dtype) < (int64_t)1 << 28, "%s: rows %lld elements apart, less than 2^28 bytes are supported", who, (long long)st);
+        SV_REQUIRE(a->T == 1 || (st >= 0 && st * elem_bytes(a->dtype) < (int64_t)1 << 28), "%s: rows %lld elements apart, less than 2^28 bytes are supported", who, (long long)st);
     return SHIVAE_OK;
 }
 

@@ -297,6 +297,88 @@ def test_streams_and_graph_replay():
         assert all(torch.equal(a, b) for a, b in zip(out, eager)), i
 
 
+@pytest.mark.parametrize("only", ["D", "dt_bias"])
+def test_selective_scan_with_one_of_its_parameters(only):
+    """D without dt_bias and the other way round, with gradients."""
+    case = (35, 2, 70, 16, 1, "f32", False, True, True, False, False)
+    v, _, softplus, dy, _ = _scan_inputs(case)
+    v["dt_bias" if only == "D" else "D"] = None
+    a = {k: _np(t) for k, t in v.items()}
+    want, scale = ref.scan(a["u"], a["dt"], a["A"], a["B"], a["C"], a["D"], None, a["dt_bias"], None, None, True, _np(dy))
+    leaves = {k: t.clone().requires_grad_(True) for k, t in v.items() if t is not None}
+    y = _scan({**{k: None for k in v}, **leaves}, None, True, False)
+    _near(y, want["y"], scale["y"], 3 * 35 + 96, "y")
+    for k, g in zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)):
+        _near(g, want[k], scale[k], 2 * (3 * 35 + 96) + 16 + 35, "d" + k)
+
+
+def test_selective_scan_without_memory():
+    """A = -inf keeps nothing of a state, and rows behind a sequence's end still leave the state as it is."""
+    mk = _Maker(21, "f32")
+    T, B, D, N = 21, 2, 64, 16
+    u, dt, Bm, Cm, s0 = mk.act(T, B, D), mk.act(T, B, D), mk.act(T, B, 1, N), mk.act(T, B, 1, N), mk.par(B, N, D)
+    A = torch.full((N, D), -float("inf"), device="cuda", requires_grad=True)
+    n = torch.tensor([17, 0], device="cuda")
+    y, last = shivae_amd.selective_scan(u, dt, A, Bm, Cm, initial_state=s0, lengths=n, return_state=True)
+    step = torch.nn.functional.softplus(dt.double())
+    want = (Cm[:, :, 0] * Bm[:, :, 0]).double().sum(-1, keepdim=True) * step * u.double()
+    scale = (Cm[:, :, 0] * Bm[:, :, 0]).double().abs().sum(-1, keepdim=True) * (step * u.double()).abs()
+    _near(y[:17, 0], want[:17, 0].cpu().numpy(), scale[:17, 0].cpu().numpy(), 64, "y")
+    assert torch.equal(last[1], s0[1]) and torch.isfinite(last).all()
+    g, = torch.autograd.grad(y.sum(), A)
+    assert torch.equal(g, torch.zeros_like(g))
+
+
+def test_refusals():
+    mk = _Maker(22, "f32")
+    T, B, D, N = 5, 2, 8, 4
+    x, w, A, Bm = mk.act(T, B, D), mk.par(4, D), -torch.exp(mk.par(N, D)), mk.act(T, B, 1, N)
+    conv, scan = shivae_amd.causal_conv, shivae_amd.selective_scan
+    cs, ss = mk.act(3, B, D), mk.par(B, N, D)
+    for f, args, kw, err in (
+            (conv, (x, mk.par(5, D)), {}, ValueError), (conv, (x, mk.par(1, D)), {}, ValueError), (conv, (x, mk.par(4, D + 1)), {}, ValueError),
+            (conv, (x, w.bfloat16()), {}, TypeError), (conv, (x, w.cpu()), {}, ValueError), (conv, (x, w), dict(activation="relu"), ValueError),
+            (conv, (x, w, mk.par(D + 1)), {}, ValueError), (conv, (x, w), dict(initial_state=cs.bfloat16()), TypeError),
+            (conv, (x, w), dict(initial_state=cs[:2]), ValueError), (conv, (x, w), dict(lengths=torch.ones(B, device="cuda")), TypeError),
+            (conv, (x, w), dict(lengths=torch.ones(B, dtype=torch.int32)), ValueError), (conv, (x, w), dict(lengths=[1, 2]), TypeError),
+            (scan, (x, x.bfloat16(), A, Bm, Bm), {}, TypeError), (scan, (x, x[:4], A, Bm, Bm), {}, ValueError),
+            (scan, (x, x, mk.par(65, D), mk.act(T, B, 1, 65), mk.act(T, B, 1, 65)), {}, ValueError), (scan, (x, x, A, Bm[:, :, 0], Bm), {}, ValueError),
+            (scan, (x, x, A, mk.act(T, B, 3, N), mk.act(T, B, 3, N)), {}, ValueError), (scan, (x, x, A, Bm, Bm[..., :3]), {}, ValueError),
+            (scan, (x, x, A.double(), Bm, Bm), {}, TypeError), (scan, (x, x, A, Bm, Bm), dict(initial_state=ss.bfloat16()), TypeError),
+            (scan, (x, x, A, Bm, Bm), dict(z=x.cpu()), ValueError),
+            (shivae_amd.causal_conv_step, (x[0], w), dict(state=cs, state_out=cs[:2]), ValueError),
+            (shivae_amd.causal_conv_step, (x[0], w.requires_grad_(True)), dict(state=cs), RuntimeError),
+            (shivae_amd.selective_scan_step, (x[0], x[0], A, Bm[0], Bm[0], ss.transpose(0, 1).contiguous().transpose(0, 1)), {}, ValueError),
+            (shivae_amd.selective_scan_step, (x[0], x[0], A, Bm[0], Bm[0], None), {}, TypeError)):
+        with pytest.raises(err):
+            f(*args, **kw)
+    big = mk.par(B + 1, N, D)  # a new state that overlaps the old one by all but one sequence
+    with pytest.raises(ValueError, match="overlaps"):
+        shivae_amd.selective_scan_step(x[0], x[0], A, Bm[0], Bm[0], big[:B], state_out=big[1:])
+
+
+def test_two_passes_of_states_in_a_graph():
+    """More than 16 states: the backward pass keeps adjoints in dynamic LDS, captured and replayed."""
+    v, n, softplus, dy, _ = _scan_inputs((50, 2, 40, 40, 1, "bf16", True, True, True, False, False))
+
+    def train():
+        u = v["u"].detach().requires_grad_(True)
+        y = _scan({**v, "u": u}, None, True, False)
+        return [y.detach(), torch.autograd.grad(y, u, dy)[0]]
+
+    train()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = train()
+    for i in range(3):
+        v["u"].mul_(-0.7)
+        g.replay()
+        eager = train()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager)), i
+
+
 def test_state_offsets_past_32_bits():
     """States of more than 2^32 bytes and 2^31 elements apart in one tensor: the last sequence is computed like the first."""
     B, D, N = 33, 1 << 20, 64  # 2^31 + 2^26 fp32 states, 8.6 GB
