@@ -88,8 +88,6 @@ struct Weigh {
     }
 };
 
-__device__ __forceinline__ u64 shfl_u64(u64 v, int lane) { return (u64)__shfl((long long)v, lane, 64); }
-__device__ __forceinline__ u64 shfl_up_u64(u64 v, int d) { return (u64)__shfl_up((long long)v, d, 64); }
 // The sum over the wave's lanes, in every lane: rotations within rows of 16 lanes, then exchanges of rows (no LDS round trips).
 template <int CTRL>
 __device__ __forceinline__ u64 ror_add(u64 v) {
@@ -106,6 +104,24 @@ __device__ __forceinline__ u64 wave_sum(u64 v) {
     l = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
     h = __builtin_amdgcn_permlane32_swap((unsigned)(v >> 32), (unsigned)(v >> 32), false, false);
     return ((u64)h[0] << 32 | l[0]) + ((u64)h[1] << 32 | l[1]);
+}
+
+// The sum over lanes 0 to this one: shifts within rows of 16 lanes (row_shr, 0 from outside), then the rows in front.
+template <int CTRL>
+__device__ __forceinline__ u64 shr_add(u64 v) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0u, (unsigned)v, CTRL, 0xf, 0xf, false), hi = __builtin_amdgcn_update_dpp(0u, (unsigned)(v >> 32), CTRL, 0xf, 0xf, false);
+    return v + ((u64)hi << 32 | lo);
+}
+__device__ __forceinline__ u64 lane_u64(u64 v, int l) {
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)v, l);
+}
+__device__ __forceinline__ u64 wave_scan(u64 v, int lane) {
+    v = shr_add<0x111>(v);
+    v = shr_add<0x112>(v);
+    v = shr_add<0x114>(v);
+    v = shr_add<0x118>(v);
+    const u64 r0 = lane_u64(v, 15), r1 = lane_u64(v, 31), r2 = lane_u64(v, 47);
+    return v + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
 }
 
 // ------------------------------------------------------------------------------------------------ a workgroup per row
@@ -184,19 +200,15 @@ struct Sampler {
 
     // Exclusive sum of v over the workgroup's threads, and the whole sum.  Ends with a barrier behind the last read.
     __device__ __forceinline__ u64 scan(u64 v, u64& total) {
-        u64 in = v;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const u64 o = shfl_up_u64(in, d);
-            if (lane >= d) in += o;
-        }
+        const u64 in = wave_scan(v, lane);
         if (NWV == 1) {
-            total = shfl_u64(in, 63);
+            total = lane_u64(in, 63);
             return in - v;
         }
         if (lane == 63) s.wave[wv] = in;
         __syncthreads();
         u64 before = 0, all = 0;
+#pragma unroll
         for (int i = 0; i < NWV; ++i) {
             const u64 w = s.wave[i];
             if (i < wv) before += w;
@@ -238,29 +250,22 @@ struct Sampler {
         return at;
     }
 
-    // list[0, n) into descending order (entries differ, but for zeros, which end up behind the rest).  Short lists by counting what is
-    // larger, at two barriers; longer ones, padded to a power of two with zeros, by a bitonic network, a barrier for each of its steps.
+    // list[0, n) into descending order (entries differ, but for zeros, which end up behind the rest).  Up to 128 entries by counting what
+    // is larger, at two barriers and by the waves that hold some; longer lists, padded to a power of two with zeros, by a bitonic network.
     __device__ __forceinline__ void sort(int n) {
-        constexpr int R = 1024 / NT > 1 ? 2 : 1;  // elements per thread
-        if (n <= R * NT && n <= 1024) {
-            u64 e[R];
-            int rank[R];
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int i = tid + r * NT;
-                e[r] = i < n ? s.list[i] : 0;
-                rank[r] = 0;
-            }
+        if (n <= 128 && n <= NT) {
+            u64 e = 0;
+            int rank = 0;
+            if (tid < n) {
+                e = s.list[tid];
 #pragma unroll 4
-            for (int j = 0; j < n; ++j) {
-                const u64 o = s.list[j];
-#pragma unroll
-                for (int r = 0; r < R; ++r) rank[r] += o > e[r] || (o == e[r] && j < tid + r * NT);
+                for (int j = 0; j < n; ++j) {
+                    const u64 o = s.list[j];
+                    rank += o > e || (o == e && j < tid);
+                }
             }
             __syncthreads();
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-                if (tid + r * NT < n) s.list[rank[r]] = e[r];
+            if (tid < n) s.list[rank] = e;
             __syncthreads();
             return;
         }
@@ -376,54 +381,51 @@ struct Sampler {
             prefix |= (unsigned)(255 - d) << shift;
             mask |= 255u << shift;
         }
-        // Equal values from here on: which of them in index order
+        // Equal values from here on: which of them in index order.  (Those that an earlier cut dropped lie behind its own place.)
         const float x0 = of_key(prefix);
         const u64 w = weight(x0), nth = w ? (g - before) / w : 0;
+        const bool tie = last && of_key((unsigned)(last >> 32)) == x0;
+        upto = tie ? (int)(0xffffffffu - (unsigned)last) : 0x7fffffff;
+        low = x0;
         u64 bf, total;
         float xv;
-        const int idx = locate([&](float x, int i) { return x == x0 && place(x, i) >= last; }, [](float) { return (u64)1; }, [&](u64) { return nth; }, bf, total, xv);
+        const int idx = locate([&](float x) { return (u64)(x == x0); }, [&](u64) { return nth; }, bf, total, xv);
         return place(x0, idx < 0 ? V - 1 : idx);
     }
 
-    // The first index, in index order, at which the running sum of weight(x), over what take(x, index) holds of, exceeds goal(total); -1
-    // if none.  Sums of 64-vector segments first, then one wave looks into the segment.  A wave whose segment is at most half taken
-    // first puts those elements side by side (in its part of the list), so that weights are computed for full waves of them.
-    template <class T, class W, class G>
-    __device__ __forceinline__ int locate(T take, W weight, G goal, u64& before, u64& total, float& value) {
+    // What the draw takes: above low, and at low up to index `upto`.
+    float low;
+    int upto;
+    __device__ __forceinline__ bool takes(float x, int idx) const { return x > low || (x == low && idx <= upto); }
+
+    // The first index, in index order, at which the running sum of weight(x), over what takes(x, index) holds of, exceeds goal(total); -1
+    // if none.  Sums of 64-vector segments first, then one wave looks into the segment.  Where few elements are taken a lane computes
+    // weights for its own only, one in each round.
+    template <class W, class G>
+    __device__ __forceinline__ int locate(W weight, G goal, u64& before, u64& total, float& value) {
         const int nseg = (nvec + 63) / 64;
-        constexpr int PER = 64 * VE;  // elements of a segment
-        float* mine = reinterpret_cast<float*>(s.list) + wv * PER;
-        constexpr bool room = (size_t)NWV * PER * sizeof(float) <= sizeof(s.list);
         sweep([&](int i, const float (&x)[VE]) {
-            bool in[VE];
-            int all = 0;  // elements taken by the wave
+            unsigned m = 0;
 #pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                in[k] = take(x[k], i * VE + k - off);
-                all += __popcll(__ballot(in[k]));
-            }
+            for (int k = 0; k < VE; ++k) m |= takes(x[k], i * VE + k - off) ? 1u << k : 0u;
             u64 sum = 0;
-            if (room && all <= PER / 2) {
-                int at = 0;
+            if (!__any(__popc(m) > VE / 2)) {
+                while (__any(m != 0)) {
+                    float v = x[0];
 #pragma unroll
-                for (int k = 0; k < VE; ++k) {
-                    const u64 on = __ballot(in[k]);
-                    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(on >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)on, 0));
-                    if (in[k]) mine[at + before] = x[k];
-                    at += __popcll(on);
+                    for (int k = 1; k < VE; ++k) v = (m & ((1u << k) - 1)) ? v : x[k];  // the last k with nothing taken in front of it
+                    const u64 w = weight(v);
+                    if (m) sum += w;
+                    m &= m - 1;
                 }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 4
-                for (int j = lane; j < all; j += 64) sum += weight(mine[j]);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             } else {
                 u64 w[VE];
 #pragma unroll
                 for (int k = 0; k < VE; ++k) w[k] = weight(x[k]);
 #pragma unroll
-                for (int k = 0; k < VE; ++k) sum += in[k] ? w[k] : 0;
+                for (int k = 0; k < VE; ++k) sum += m >> k & 1 ? w[k] : 0;
             }
-            if (all) sum = wave_sum(sum);
+            if (__any(sum != 0)) sum = wave_sum(sum);
             if (lane == 0) s.hist[i >> 6] = sum;
         });
         __syncthreads();
@@ -438,15 +440,10 @@ struct Sampler {
             if (i < nvec) get(i, x);
 #pragma unroll
             for (int k = 0; k < VE; ++k) {
-                w[k] = i < nvec && take(x[k], i * VE + k - off) ? weight(x[k]) : 0;
+                w[k] = i < nvec && takes(x[k], i * VE + k - off) ? weight(x[k]) : 0;
                 sum += w[k];
             }
-            u64 in = sum;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const u64 o = shfl_up_u64(in, d);
-                if (lane >= d) in += o;
-            }
+            const u64 in = wave_scan(sum, lane);
             u64 run = before + in - sum;
             if (run <= g && run + sum > g) {
                 bool open = true;
@@ -570,11 +567,15 @@ struct Sampler {
                 if (bp < NB - 1) last = resolve(bp, bf, g, fix);
             }
             // 4. the draw over the row
-            const float low = of_key((unsigned)(last >> 32));
-            const bool all = last == 0;
-            const float least = smallest(wt);
+            low = smallest(wt);
+            upto = 0x7fffffff;
+            const float cut = last ? of_key((unsigned)(last >> 32)) : -INFINITY;
+            if (cut >= low) {
+                low = cut;
+                upto = (int)(0xffffffffu - (unsigned)last);
+            }
             idx = locate(
-                [&](float x, int i) { return (all || x > low || (x == low && place(x, i) >= last)) && x >= least; }, fix,
+                fix,
                 [&](u64 t) { return draw(q.u, t); }, before, total, xv);
             if (idx < 0) {  // (not reached: the largest is always kept)
                 idx = first_equal(top);
