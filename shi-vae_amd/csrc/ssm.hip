@@ -151,7 +151,10 @@ struct RowRegs {
     // as fp32; rows at and behind `left` and states at and behind N are 0
     __device__ __forceinline__ void get(float (&v)[S], int s0, int N, int left, int lane) const {
 #pragma unroll
-        for (int j = 0; j < S; ++j) v[j] = (lane & 15) < left && s0 + j < N ? elem_f(e.v[j]) : 0.f;
+        for (int j = 0; j < S; ++j) v[j] = elem_f(e.v[j]);
+        if (left >= TT && N % (4 * S) == 0) return;  // (a whole tile of whole states: uniform, and the usual case)
+#pragma unroll
+        for (int j = 0; j < S; ++j) v[j] = (lane & 15) < left && s0 + j < N ? v[j] : 0.f;
     }
 };
 
@@ -267,12 +270,20 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
         if (a.softplus)
 #pragma unroll
             for (int k = 0; k < 4; ++k) s[k] = seq_softplus(s[k]);
+        float su[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) su[k] = s[k] * ku[k];
+        if (left < TT)  // rows behind the sequence leave the state as it is
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool in = 4 * k + g4 < left;
+                s[k] = in ? s[k] : 0.f;
+                su[k] = in ? su[k] : 0.f;
+            }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const bool in = 4 * k + g4 < left;  // rows behind the sequence leave the state as it is
-            s[k] = in ? s[k] : 0.f;
             if (FIRST) total += s[k];
-            row[4 * k + g4][lane & 15] = make_float2(s[k], in ? s[k] * ku[k] : 0.f);
+            row[4 * k + g4][lane & 15] = make_float2(s[k], su[k]);
         }
         nB.get(vB, g4 * S, a.N, left, lane);
         if (!FIRST) nC.get(vC, g4 * S, a.N, left, lane);
