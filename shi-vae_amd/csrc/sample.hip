@@ -5,7 +5,7 @@
 //   token = the first index i, in index order, with  sum_{kept j <= i} w_j > u * sum_{kept j} w_j
 //
 // Which category is drawn hangs on comparisons of long sums, and 16-bit logits have long runs of equal values, whose errors add up
-// in step.  So a weight is computed in 64 bits (a polynomial for 2^f, error below 2^-36) and held as a multiple of 2^-43 of the
+// in step.  So a weight is computed in 64 bits (a polynomial for 2^f, error below 2^-38) and held as a multiple of 2^-43 of the
 // largest: sums of these are exact, independent of order (integer LDS atomics included), and fit 63 bits for 2^20 categories.  A
 // weight below 2^-44 of the largest is 0 and is never drawn.  Order is by the logits' own bits, never by rounded quotients.
 //
@@ -41,34 +41,35 @@ __device__ __forceinline__ RowParams row_params(const shivae_sample_args& a, int
     return q;
 }
 
-// A logit as it is compared: NaN counts as -inf, -0 as 0.
-__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY) + 0.f; }
-// Unsigned keys in the order of the values, and back.
+// A logit as it is compared: NaN counts as -inf.
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }
+// Unsigned keys in the order of the values (-0 as 0), and back.
 __device__ __forceinline__ unsigned key_of(float x) {
-    const unsigned b = __float_as_uint(x);
+    const unsigned b = __float_as_uint(x + 0.f);
     return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
 constexpr int kFix = 43;
-// 2^(y + shift) for -900 <= y <= 0: 2^f = sum (f ln 2)^k / k!, |f| <= 1/2; the first dropped term is (0.3466)^10 / 10! = 7e-12 = 2^-37.
-// Adding 1.5 2^52 rounds y to a whole number and leaves it in the low word; the exponent is added to the high word (v_rndne_f64,
-// v_ldexp_f64 and the conversion cost several fused operations each).
-__device__ __forceinline__ double exp2_f64(double y, int shift) {
-    constexpr double magic = 6755399441055744.0;
+// 2^(y + SHIFT) for -900 <= y <= 0.  2^f = 1 + f P(f), |f| <= 1/2, where P, of degree 7, meets (2^f - 1) / f at the eight Chebyshev
+// nodes of the interval: within 2.2e-12 = 2^-38.7 (the Taylor series needs two terms more for that).  Adding 1.5 2^52 + SHIFT rounds y to a
+// whole number and leaves it, SHIFT larger, in the low word, which is added to the exponent (v_rndne_f64, v_ldexp_f64 and the conversion
+// cost several fused operations each).
+template <int SHIFT>
+__device__ __forceinline__ double exp2_f64(double y) {
+    constexpr double magic = 6755399441055744.0 + SHIFT;
     const double t = y + magic, f = y - (t - magic);
-    double p = 1.0178086009239699e-07;
-    p = fma(p, f, 1.3215486790144309e-06);
-    p = fma(p, f, 1.5252733804059841e-05);
-    p = fma(p, f, 1.5403530393381608e-04);
-    p = fma(p, f, 1.3333558146428443e-03);
-    p = fma(p, f, 9.6181291076284772e-03);
-    p = fma(p, f, 5.5504108664821580e-02);
-    p = fma(p, f, 2.4022650695910072e-01);
-    p = fma(p, f, 6.9314718055994531e-01);
+    double p = 1.3250805517502250e-06;
+    p = fma(p, f, 1.5303700711365693e-05);
+    p = fma(p, f, 1.5403475186530786e-04);
+    p = fma(p, f, 1.3333478473685416e-03);
+    p = fma(p, f, 9.6181291352361396e-03);
+    p = fma(p, f, 5.5504109063258665e-02);
+    p = fma(p, f, 2.4022650695888503e-01);
+    p = fma(p, f, 6.9314718055683244e-01);
     p = fma(p, f, 1.0);
     const u64 b = (u64)__double_as_longlong(p);
-    const unsigned hi = (unsigned)(b >> 32) + (((unsigned)__double_as_longlong(t) + (unsigned)shift) << 20);
+    const unsigned hi = (unsigned)(b >> 32) + ((unsigned)__double_as_longlong(t) << 20);
     return __longlong_as_double((long long)((u64)hi << 32 | (unsigned)b));
 }
 // The weight of x as a multiple of 2^-43: adding 2^52 rounds to whole numbers and leaves them in the mantissa.
@@ -84,7 +85,7 @@ struct Weigh {
     __device__ __forceinline__ bool enough(float x) const { return log2w(x) >= least; }  // min-p
     // No branch: eight elements' chains of dependent operations run side by side.  -inf (and -inf * 0) become 2^-200, which rounds to 0.
     __device__ __forceinline__ u64 fix(float x) const {
-        return (u64)__double_as_longlong(exp2_f64(fmax(log2w(x), -200.0), kFix) + 4503599627370496.0) & 0xfffffffffffffull;
+        return (u64)__double_as_longlong(exp2_f64<kFix>(fmax(log2w(x), -200.0)) + 4503599627370496.0) & 0xfffffffffffffull;
     }
 };
 
@@ -283,7 +284,13 @@ struct Sampler {
                         s.list[b] = x;
                     }
                 }
-                __syncthreads();
+                // A wave's 64 pairs lie in 128 entries that are its own in every step with j <= 64.
+                if (j > 64 || (j > 1 ? j >> 1 : k) > 64) {
+                    __syncthreads();
+                } else {
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                }
             }
     }
 
@@ -398,36 +405,45 @@ struct Sampler {
     int upto;
     __device__ __forceinline__ bool takes(float x, int idx) const { return x > low || (x == low && idx <= upto); }
 
+    // The sum over the wave's elements whose bits in m are set goes to the sum of their segment, 64 vectors.  Where few elements are taken a
+    // lane computes weights for its own only, one in each round.
+    template <class W>
+    __device__ __forceinline__ void segment_sum(int i, const float (&x)[VE], unsigned m, W weight) {
+        u64 sum = 0;
+        if (!__any(__popc(m) > VE / 2)) {
+            while (__any(m != 0)) {
+                float v = x[0];
+#pragma unroll
+                for (int k = 1; k < VE; ++k) v = (m & ((1u << k) - 1)) ? v : x[k];  // the last k with nothing taken in front of it
+                const u64 w = weight(v);
+                if (m) sum += w;
+                m &= m - 1;
+            }
+        } else {
+            u64 w[VE];
+#pragma unroll
+            for (int k = 0; k < VE; ++k) w[k] = weight(x[k]);
+#pragma unroll
+            for (int k = 0; k < VE; ++k) sum += m >> k & 1 ? w[k] : 0;
+        }
+        if (__any(sum != 0)) sum = wave_sum(sum);
+        if (lane == 0) s.hist[i >> 6] = sum;
+    }
     // The first index, in index order, at which the running sum of weight(x), over what takes(x, index) holds of, exceeds goal(total); -1
-    // if none.  Sums of 64-vector segments first, then one wave looks into the segment.  Where few elements are taken a lane computes
-    // weights for its own only, one in each round.
+    // if none.  Sums of segments first, then one wave looks into the segment.
     template <class W, class G>
     __device__ __forceinline__ int locate(W weight, G goal, u64& before, u64& total, float& value) {
-        const int nseg = (nvec + 63) / 64;
         sweep([&](int i, const float (&x)[VE]) {
             unsigned m = 0;
 #pragma unroll
             for (int k = 0; k < VE; ++k) m |= takes(x[k], i * VE + k - off) ? 1u << k : 0u;
-            u64 sum = 0;
-            if (!__any(__popc(m) > VE / 2)) {
-                while (__any(m != 0)) {
-                    float v = x[0];
-#pragma unroll
-                    for (int k = 1; k < VE; ++k) v = (m & ((1u << k) - 1)) ? v : x[k];  // the last k with nothing taken in front of it
-                    const u64 w = weight(v);
-                    if (m) sum += w;
-                    m &= m - 1;
-                }
-            } else {
-                u64 w[VE];
-#pragma unroll
-                for (int k = 0; k < VE; ++k) w[k] = weight(x[k]);
-#pragma unroll
-                for (int k = 0; k < VE; ++k) sum += m >> k & 1 ? w[k] : 0;
-            }
-            if (__any(sum != 0)) sum = wave_sum(sum);
-            if (lane == 0) s.hist[i >> 6] = sum;
+            segment_sum(i, x, m, weight);
         });
+        return locate_in_sums(weight, goal, before, total, value);
+    }
+    template <class W, class G>
+    __device__ __forceinline__ int locate_in_sums(W weight, G goal, u64& before, u64& total, float& value) {
+        const int nseg = (nvec + 63) / 64;
         __syncthreads();
         u64 g = 0;
         const int seg = first_beyond(nseg, [&](int i) { return s.hist[i]; }, [&](u64 t) { return g = goal(t); }, before, total);
@@ -463,6 +479,44 @@ struct Sampler {
         value = __uint_as_float((unsigned)s.found[1]);
         __syncthreads();
         return idx;
+    }
+
+    // Where the lead ends in bin b, in front of which it holds all (weight `before`): one pass sums what is taken of those bins by segments and
+    // lists bin b; what the lead holds of the list is added to the segments.  Sets `last`; false, with nothing done, if the list is too short.
+    template <class W>
+    __device__ __forceinline__ bool lead_sums(int b, u64 before, u64 g, W weight) {
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+        sweep([&](int i, const float (&x)[VE]) {
+            unsigned m = 0, e = 0;
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                const int bk = bin(x[k]);
+                m |= bk < b && x[k] >= low ? 1u << k : 0u;
+                e |= bk == b && place(x[k], i * VE + k - off) >= last ? 1u << k : 0u;
+            }
+            segment_sum(i, x, m, weight);
+            if (!e) return;
+            int at = atomicAdd(&s.count, __popc(e));
+#pragma unroll
+            for (int k = 0; k < VE; ++k)
+                if ((e >> k & 1) && at < CAP) s.list[at++] = place(x[k], i * VE + k - off);
+        });
+        __syncthreads();
+        const int n = s.count;
+        __syncthreads();
+        if (n > CAP) return false;
+        sort(n);
+        u64 bf, total;
+        const int at = first_beyond(n, [&](int i) { return weight(of_key((unsigned)(s.list[i] >> 32))); }, [&](u64) { return g - before; }, bf, total);
+        if (n) last = s.list[min(at, n - 1)];
+        for (int i = tid; i <= min(at, n - 1); i += NT) {
+            const float x = of_key((unsigned)(s.list[i] >> 32));
+            const int idx = (int)(0xffffffffu - (unsigned)s.list[i]);
+            if (x >= low) atomicAdd(&s.hist[(idx + off) / VE >> 6], weight(x));
+        }
+        __syncthreads();
+        return true;
     }
 
     __device__ __forceinline__ float block_max(float v) {
@@ -559,24 +613,30 @@ struct Sampler {
             idx = (int)(0xffffffffu - (unsigned)(e >> 32));
             xv = of_key((unsigned)e);
         } else {
-            // 3. top-p over the row: the bin in which the lead ends
+            // 3. top-p over the row: the bin in which the lead ends, then its last element
+            low = smallest(wt);
+            upto = 0x7fffffff;
+            bool summed = false;
             if (q.top_p < 1.f) {
                 fill(NB, [&](float x, int i) { return last && place(x, i) < last ? -1 : has_weight(x); }, fix);
                 u64 bf, g = 0;
                 const int bp = first_beyond(NB - 1, [&](int i) { return s.hist[i]; }, [&](u64 t) { return g = lead(q.top_p, t); }, bf, total);
-                if (bp < NB - 1) last = resolve(bp, bf, g, fix);
+                if (bp < NB - 1) {
+                    const float least = low;
+                    summed = lead_sums(bp, bf, g, fix);
+                    if (!summed) last = resolve(bp, bf, g, fix);
+                    low = least;
+                    upto = 0x7fffffff;
+                }
             }
             // 4. the draw over the row
-            low = smallest(wt);
-            upto = 0x7fffffff;
             const float cut = last ? of_key((unsigned)(last >> 32)) : -INFINITY;
             if (cut >= low) {
                 low = cut;
                 upto = (int)(0xffffffffu - (unsigned)last);
             }
-            idx = locate(
-                fix,
-                [&](u64 t) { return draw(q.u, t); }, before, total, xv);
+            const auto goal = [&](u64 t) { return draw(q.u, t); };
+            idx = summed ? locate_in_sums(fix, goal, before, total, xv) : locate(fix, goal, before, total, xv);
             if (idx < 0) {  // (not reached: the largest is always kept)
                 idx = first_equal(top);
                 xv = top;
