@@ -252,11 +252,16 @@ int launch_sum_parts(const float* part, int64_t n, int cols, float* mid, float* 
     return SHIVAE_OK;
 }
 
-static int conv_run(const shivae_conv_args& a, int vec, int lo) {
-    // Time steps per thread: as many as leave about eight waves for every SIMD of the card, between `lo` and 64.
+// Time steps per thread.  Forward 16: longer runs read fewer rows twice, but leave fewer loads in flight (us, runs of 16 / 32 / 64: T 2048,
+// B 16, D 2048, bf16 49 / 49 / 55; T 1000, B 64, D 256, fp32 23 / 24 / 30; T 256, B 4, D 512 10.7 / 12.8 / 22; T 4096, B 64 runs of 16 / 64
+// 421 / 447).  Backward a run writes partial sums of the parameters' gradients, (W + 1) D fp32 numbers, as much as ten bf16 rows: as long as
+// two waves are left for every SIMD, up to 256 (with 8 / 4 / 2 waves: 205 / 172 / 161; 60 / 61 / 52; 26 in all; and T 4096, B 64, up to
+// 64 / 256: 1136 / 1028).
+static int conv_run(const shivae_conv_args& a, int vec, bool bwd) {
     const int64_t seqs = (int64_t)a.B * ceil_div(a.D, vec);
-    int run = lo;
-    while (run < 64 && seqs * ceil_div(a.T, run * 2) >= 1024 * 8 * 64) run *= 2;
+    int run = 16;
+    if (bwd)
+        while (run < 256 && seqs * ceil_div(a.T, run * 2) >= 1024 * 2 * 64) run *= 2;
     while (ceil_div(a.T, run) > 65535) run *= 2;
     return run;
 }
@@ -301,7 +306,7 @@ int shivae_causal_conv_fwd(const shivae_conv_args* args, shivae_stream stream) {
     const shivae_conv_args& a = *args;
     SV_REQUIRE(a.y, "causal_conv_fwd: y is required");
     const int v = conv_vec(a, false);
-    ConvP p{a, ceil_div(a.D, v), conv_run(a, v, 16), 0, nullptr};
+    ConvP p{a, ceil_div(a.D, v), conv_run(a, v, false), 0, nullptr};
     p.nrun = ceil_div(a.T, p.run);
     SV_REQUIRE(!a.state || a.state != a.state_out || p.nrun == 1, "causal_conv_fwd: the state can be updated in place for up to %d time steps only", p.run);
     const dim3 grid((unsigned)(((int64_t)a.B * p.nvec + 255) / 256), p.nrun);
@@ -316,7 +321,7 @@ int shivae_causal_conv_fwd(const shivae_conv_args* args, shivae_stream stream) {
 size_t shivae_causal_conv_bwd_ws(const shivae_conv_args* args) {
     if (conv_check(args, "causal_conv_bwd_ws") != SHIVAE_OK) return 0;
     // (runs are shortest, and partials most, where a thread owns eight channels)
-    const int64_t n = (int64_t)ceil_div(args->T, conv_run(*args, 8, 16)) * args->B, cols = (int64_t)(args->W + 1) * args->D;
+    const int64_t n = (int64_t)ceil_div(args->T, conv_run(*args, 8, true)) * args->B, cols = (int64_t)(args->W + 1) * args->D;
     return ((size_t)n * cols + sum_parts_floats(n, cols)) * sizeof(float);
 }
 
@@ -330,7 +335,7 @@ int shivae_causal_conv_bwd(const shivae_conv_args* args, void* ws_dev, size_t ws
     SV_REQUIRE(ws_dev && ws_bytes >= need, "causal_conv_bwd: workspace of %zu bytes is smaller than %zu", ws_bytes, need);
     SV_REQUIRE(aligned_to(ws_dev, 16), "causal_conv_bwd: the workspace must be 16-byte aligned");
     const int v = conv_vec(a, true);
-    ConvP p{a, ceil_div(a.D, v), conv_run(a, v, 16), 0, static_cast<float*>(ws_dev)};
+    ConvP p{a, ceil_div(a.D, v), conv_run(a, v, true), 0, static_cast<float*>(ws_dev)};
     p.nrun = ceil_div(a.T, p.run);
     const dim3 grid((unsigned)(((int64_t)a.B * p.nvec + 255) / 256), p.nrun);
     hipStream_t s = static_cast<hipStream_t>(stream);
