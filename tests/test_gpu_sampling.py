@@ -74,6 +74,35 @@ def test_runs_of_equal_logits(V):
             _check(lg.bfloat16(), torch.rand(4, device="cuda", generator=gen), **kw)
 
 
+@pytest.mark.parametrize("rows, V, dtype", [(2048, 513, "bf16"), (2050, 2049, "f32"), (2048, 4096, "bf16"), (515, 8193, "f16"), (512, 20001, "bf16")])
+def test_many_long_rows(rows, V, dtype):
+    """The choice of threads goes by rows as well: as many rows as change it, with runs of equal values longer than any list among them."""
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    lg = _logits(gen, rows, V, dtype)
+    lg[1] = 0.0
+    lg[2] = (lg[2] > 0).to(lg.dtype)
+    lg[3, ::2] = -float("inf")
+    lg[4] = torch.randint(0, 3, (V,), device="cuda", generator=gen).to(lg.dtype) * 0.01
+    keep = torch.arange(0, rows, max(1, rows // 60), device="cuda")
+    keep = torch.cat([torch.arange(5, device="cuda"), keep[1:], torch.tensor([rows - 1], device="cuda")])
+    for kw in (dict(), dict(top_k=50, top_p=0.9), dict(top_k=V // 2 + 1, top_p=0.6), dict(top_p=0.95, min_p=0.02), dict(top_k=V - 5)):
+        u = torch.rand(rows, device="cuda", generator=gen)
+        tok = shivae_amd.sample_categories(lg, u, **kw)
+        want = _check(lg[keep], u[keep], **kw)  # (few rows: other threads, and the definition)
+        torch.testing.assert_close(tok[keep], want, rtol=0, atol=0)
+
+
+def test_a_lead_that_ends_where_top_k_does():
+    """top-k's last element, the lead's last element and min-p's limit in one bin, in rows that start off a 16-byte boundary."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    V = 20001
+    lg = _logits(gen, 7, V + 2, "bf16", spread=0.001)[:, 1:V + 1]
+    lg[:, ::3] = torch.where(torch.rand(7, V, device="cuda", generator=gen) < 0.5, 1.0, 1.0078125).bfloat16()[:, ::3]
+    for kw in (dict(top_k=5000, top_p=0.999), dict(top_k=6000, top_p=0.5, min_p=0.995), dict(top_k=6700, top_p=0.9999, min_p=0.2), dict(top_p=0.8, min_p=0.3)):
+        for u in (0.0, 0.5, 1.0 - 2.0 ** -24):
+            _check(lg, torch.full((7,), u, device="cuda"), **kw)
+
+
 @pytest.mark.parametrize("V", [7, 64, 90, 1500, 21000])
 def test_masked_and_non_finite_logits(V):
     gen = torch.Generator(device="cuda").manual_seed(3)
