@@ -6,6 +6,8 @@
 // A thread owns one 16-byte group of channels of one sequence and a run of time steps, and keeps the window of the last
 // W - 1 rows in registers, so that a row is read once per run (the W - 1 rows in front of a run are read again by the run
 // behind them).  Neighbouring threads own neighbouring channels: every access is a contiguous 1 KiB per wave.
+// Measured (W 4, silu): T 2048, B 16, D 2048, bf16 50 us, 5.4 TB/s, as fast as a copy; T 1000, B 64, D 256, fp32 18 us forward, 35 backward,
+// and 2 x 5 for the partial sums.
 #include <algorithm>
 
 #include "common.h"

@@ -9,12 +9,15 @@
 // largest: sums of these are exact, independent of order (integer LDS atomics included), and fit 63 bits for 2^20 categories.  A
 // weight below 2^-44 of the largest is 0 and is never drawn.  Order is by the logits' own bits, never by rounded quotients.
 //
+// Measured (us): 256 x 131072, bf16, top-p 0.95 133, with min-p 0.01 115, top-k 50 55, no cut 62, the largest alone 24; 1 x 32768, top-k 50
+// and top-p 21; 102400 rows of 8 9.  Where it hurts: a row stays on one compute unit, 1 x 131072 with top-p takes 118 us.
+//
 // A row is a workgroup's.  No row is sorted: top-k and top-p need the last element they keep.  A histogram of (max - x) /
 // temperature over the range that has weight (counts, or sums of weights) finds the bin it lies in; the elements of that bin -- or
 // of all bins up to it, when they are few, which leaves nothing of the row to read again -- go to a list in LDS that is sorted.  A
 // bin too full for the list (runs of equal values) is resolved by four 8-bit digits of the key instead.  Bound by the row's reads
-// for few kept elements (the row stays in L2 between the passes) and by the 64-bit exponentials, about 20 instructions each, for
-// many.
+// for few kept elements (the row stays in L2 between the passes) and by vector instructions for many: about 25 for an exponential in 64
+// bits, 100 per category in all with top-p.
 #include "common.h"
 #include "elem.h"
 
@@ -406,7 +409,8 @@ struct Sampler {
     __device__ __forceinline__ bool takes(float x, int idx) const { return x > low || (x == low && idx <= upto); }
 
     // The sum over the wave's elements whose bits in m are set goes to the sum of their segment, 64 vectors.  Where few elements are taken a
-    // lane computes weights for its own only, one in each round.
+    // lane computes weights for its own only, one in each round.  (256 x 131072, us, no cut / min-p 0.01 / top-p 0.3: 62 / 49 / 98; always all
+    // weights 62 / 64 / 109, always rounds 91 / 48 / 98.)
     template <class W>
     __device__ __forceinline__ void segment_sum(int i, const float (&x)[VE], unsigned m, W weight) {
         u64 sum = 0;

@@ -355,7 +355,8 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
 }
 
 // One row.  A thread owns V neighbouring channels of one sequence and walks the states: the fp32 state is read and written
-// once, 16 bytes a lane, and is nearly all of the traffic.
+// once, 16 bytes a lane, and is nearly all of the traffic: B 256, D 2048, N 16, bf16: 16.4 us for 67 MB of
+// it, 4.1 TB/s.
 template <class E, int V>
 __global__ __launch_bounds__(256) void ssm_token_kernel(SsmP p, int nvec) {
     const shivae_ssm_args& a = p.a;
@@ -599,6 +600,9 @@ __device__ __forceinline__ Sums<S> sum_rows(F& f, int lane) {
 // with states and decays in registers (128 of them for S = 4), then back.  More than 16 states take several passes over a tile, 4 S
 // states each, whose adjoints and sums wait in LDS.  dB and dC are sums over all channels: of the wave's 16 by sum_rows, of the
 // workgroup's four waves through LDS (the one barrier of a pass), of the workgroups by ssm_dbc_kernel.
+// Bound by vector instructions: 197 us (T 2048, B 4, D 1536, N 16, bf16, gate, 10 pieces), in which a SIMD issues 7.7e4 of them, 0.65 of its
+// time; 218 us (T 1000, B 64, D 256, fp32).  The four passes around it: ssm_fwd_kernel 50 (FIRST) and 71, ssm_bwd_first_kernel 47,
+// ssm_dbc_kernel 10.  The sums over channels by LDS atomics on floats instead (200 cycles each) took longer than all of the rest.
 template <class E, int S, bool MANY>
 __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
     constexpr int P = 4 * S;  // states of a pass
@@ -888,9 +892,11 @@ static int ssm_check(const shivae_ssm_args* a, const char* who) {
     return SHIVAE_OK;
 }
 
-// Pieces of the time axis.  A split costs the second launch's work again without y (about 0.9 of it), so it is taken only
-// where the unsplit grid leaves at least half of the card's SIMDs with one wave: then pieces of at least 64 rows until there are
-// about 1024 workgroups.
+// Pieces of the time axis.  A split costs the second launch's work again without y (0.7 of it; backward a quarter), so it is taken only
+// up to 256 workgroups, one wave a SIMD: then pieces of at least 64 rows until there are about 1024.  Measured (us, forward and backward
+// together): T 1000, B 64, D 256, fp32, 256 workgroups: split 420, not 471; T 2048, B 4, D 1536, bf16, 96 workgroups: split 385, not 932.
+// For 512 / 1024 / 1536 / 2048 workgroups: T 8192, B 1, D 2048 forward 167 / 158 / 158 / 160; the two above 427 / 421 / 416 / 424 and
+// 398 / 385 / 380 / 400.
 static void ssm_split(SsmP& p) {
     const shivae_ssm_args& a = p.a;
     p.E = a.D / a.G;
@@ -946,7 +952,7 @@ template <class E>
 static int launch_ssm_bwd(SsmP& p, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)p.tiles * p.a.B * p.np));
     const int N = p.a.N, S = N <= 4 ? 1 : N <= 8 ? 2 : 4, passes = ceil_div(N, 4 * S);
-    const size_t lds = passes > 1 ? (size_t)passes * 3 * S * 256 * sizeof(float) : 0;  // up to 48 KiB beside 28 of static
+    const size_t lds = passes > 1 ? (size_t)passes * 3 * S * 256 * sizeof(float) : 0;  // up to 48 KiB beside 57 of static
     ssm_vec(p, S);
     if (lds)  // (past the default limit of 64 KiB)
         SV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_bwd_kernel<E, 4, true>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
