@@ -132,6 +132,7 @@ __device__ __forceinline__ u64 wave_scan(u64 v, int lane) {
 template <class E, int NT, int CAP, int NB>
 struct Sampler {
     static constexpr int VE = 16 / (int)sizeof(E), NWV = NT / 64;
+    static_assert(NB >= 256 && CAP >= 128, "a digit's bins and a short row's list have to fit");
     struct Shared {
         u64 hist[NB];   // bins, or sums of 64-vector segments of the row
         u64 list[CAP];

@@ -14,6 +14,7 @@ from ctypes import byref
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version  # a state written in place that a backward pass still needs is an error there
 
 from . import _native as N
 
@@ -204,6 +205,7 @@ def causal_conv_step(x, weight, bias=None, *, state, activation=None, state_out=
     args = N.ConvArgs(1, B, D, weight.shape[0], _DTYPES[x.dtype], _conv_silu(activation), x.data_ptr(), 0, x.stride(0), weight.data_ptr(),
                       _ptr(bias), state.data_ptr(), None, y.data_ptr(), 0, D, out.data_ptr())
     _call(dev, N.lib().shivae_causal_conv_fwd, byref(args))
+    increment_version(out)
     return y
 
 
@@ -319,5 +321,6 @@ def selective_scan_step(u, dt, A, B, C, state, D=None, z=None, dt_bias=None, sof
                      B.stride(1), 0, C.stride(0), C.stride(1), A.data_ptr(), _ptr(D), _ptr(dt_bias), state.data_ptr(), None,
                      y.data_ptr(), 0, Dm, out.data_ptr())
     _call(dev, N.lib().shivae_selective_scan_fwd, byref(args), None, 0)
+    increment_version(out)
     return y
 

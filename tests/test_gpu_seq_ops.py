@@ -357,6 +357,24 @@ def test_refusals():
         shivae_amd.selective_scan_step(x[0], x[0], A, Bm[0], Bm[0], big[:B], state_out=big[1:])
 
 
+def test_a_state_that_a_backward_pass_needs_is_not_changed_unnoticed():
+    """The steps write the state behind autograd's back: a graph that holds the old one refuses its backward pass."""
+    mk = _Maker(21, "f32")
+    x, w, A, B, C = mk.act(5, 2, 8), mk.par(4, 8), -mk.par(4, 8).abs(), mk.act(5, 2, 1, 4), mk.act(5, 2, 1, 4)
+    conv_state, scan_state = mk.act(3, 2, 8), mk.par(2, 4, 8)
+    leaf = x.clone().requires_grad_(True)
+    y = shivae_amd.causal_conv(leaf, w, initial_state=conv_state)
+    z = shivae_amd.selective_scan(leaf, x, A, B, C, initial_state=scan_state)
+    shivae_amd.causal_conv_step(x[0], w, state=conv_state)
+    shivae_amd.selective_scan_step(x[0], x[0], A, B[0], C[0], scan_state)
+    for out in (y, z):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, leaf, torch.ones_like(out))
+    with torch.inference_mode():
+        state = torch.zeros(3, 2, 8, device="cuda")
+        shivae_amd.causal_conv_step(x[0], w, state=state)
+
+
 def test_two_passes_of_states_in_a_graph():
     """More than 16 states: the backward pass keeps adjoints in dynamic LDS, captured and replayed."""
     v, n, softplus, dy, _ = _scan_inputs((50, 2, 40, 40, 1, "bf16", True, True, True, False, False))
