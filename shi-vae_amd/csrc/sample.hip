@@ -9,8 +9,8 @@
 // largest: sums of these are exact, independent of order (integer LDS atomics included), and fit 63 bits for 2^20 categories.  A
 // weight below 2^-44 of the largest is 0 and is never drawn.  Order is by the logits' own bits, never by rounded quotients.
 //
-// Measured (us): 256 x 131072, bf16, top-p 0.95 133, with min-p 0.01 115, top-k 50 55, no cut 62, the largest alone 24; 1 x 32768, top-k 50
-// and top-p 21; 102400 rows of 8 9.  Where it hurts: a row stays on one compute unit, 1 x 131072 with top-p takes 118 us.
+// Measured (us): 256 x 131072, bf16, top-p 0.95 133, with min-p 0.01 115, top-k 50 35, no cut 62, the largest alone 24; 1 x 32768, top-k 50
+// 14, with top-p 15.6; 102400 rows of 8 9.  Where it hurts: a row stays on one compute unit, 1 x 131072 with top-p takes 118 us.
 //
 // A row is a workgroup's.  No row is sorted: top-k and top-p need the last element they keep.  A histogram of (max - x) /
 // temperature over the range that has weight (counts, or sums of weights) finds the bin it lies in; the elements of that bin -- or
@@ -139,6 +139,7 @@ struct Sampler {
         u64 wave[NWV + 1];
         u64 found[2];
         int count, pos;
+        int rank[128];  // 0 between sorts
     };
 
     Shared& s;
@@ -259,18 +260,25 @@ struct Sampler {
     // is larger, at two barriers and by the waves that hold some; longer lists, padded to a power of two with zeros, by a bitonic network.
     __device__ __forceinline__ void sort(int n) {
         if (n <= 128 && n <= NT) {
+            // (128 threads, or a wave, for the entries, each set of them for a part of what they are compared with)
+            constexpr int SPAN = NT < 128 ? NT : 128, PARTS = NT / SPAN;
+            const int i = tid & (SPAN - 1);
             u64 e = 0;
-            int rank = 0;
-            if (tid < n) {
-                e = s.list[tid];
+            if (i < n) {
+                e = s.list[i];
+                int rank = 0;
 #pragma unroll 4
-                for (int j = 0; j < n; ++j) {
+                for (int j = tid / SPAN; j < n; j += PARTS) {
                     const u64 o = s.list[j];
-                    rank += o > e || (o == e && j < tid);
+                    rank += o > e || (o == e && j < i);
                 }
+                atomicAdd(&s.rank[i], rank);
             }
             __syncthreads();
-            if (tid < n) s.list[rank] = e;
+            if (tid < SPAN && i < n) {
+                s.list[s.rank[i]] = e;
+                s.rank[i] = 0;
+            }
             __syncthreads();
             return;
         }
@@ -553,6 +561,7 @@ struct Sampler {
     }
 
     __device__ __forceinline__ void run(const RowParams& q, int64_t* token, float* logprob) {
+        for (int i = tid; i < 128; i += NT) s.rank[i] = 0;
         // 1. the largest
         float most = -INFINITY;
         sweep([&](int, const float (&x)[VE]) {
@@ -571,6 +580,7 @@ struct Sampler {
         if (top == INFINITY) {  // the limit of ever larger logits: those at +inf share everything
             has_inf = true;
             top = 0.f;
+            most = most == INFINITY ? 0.f : -INFINITY;
         }
         Weigh wt;
         wt.set(top, q.temperature, q.min_p);
@@ -585,14 +595,27 @@ struct Sampler {
             int bk = NB - 2;
             u64 bf = 0, total = 0, upto = 0;
             const bool small = V <= 128;  // (ranks by counting; longer rows are cheaper by the histogram: 4096 x 512, top-p, 24 us against 60)
-            if (!small && q.top_k) {
+            if (!small && q.top_k && q.top_k <= NT / 2) {
+                // top_k threads whose own largest lie in the bins up to bk: so do top_k elements.  There are not many more (0.7 NT for NT / 2, if
+                // they lie at random), and the row's histogram is not needed: 1 x 32768, top-k 50 13.9 us, not 20.2; 256 x 131072 35, not 54.
+                clear(NB);
+                const int b = has_weight(most);
+                if (b >= 0) atomicAdd(&s.hist[b], (u64)1);
+                __syncthreads();
+                bk = first_beyond(NB - 1, [&](int i) { return s.hist[i]; }, [&](u64) { return (u64)q.top_k - 1; }, bf, total);
+                if (bk < NB - 1) n = gather([&](float x, int) { return bin(x) <= bk; });
+                if (n > CAP) n = -1;
+            }
+            if (n < 0 && !small && q.top_k) {
                 fill(NB, [&](float x, int) { return has_weight(x); }, one);
                 bk = first_beyond(NB - 1, [&](int i) { return s.hist[i]; }, [&](u64) { return (u64)q.top_k - 1; }, bf, total);
                 // (fewer than top_k elements of any weight: top-k keeps them all)
                 upto = bk < NB - 1 ? bf + s.hist[bk] : total;
             }
-            if (small || (q.top_k && upto <= CAP)) n = gather([&](float x, int) { return bin(x) <= min(bk, NB - 2); });
-            else if (q.top_k && bk < NB - 1) last = resolve(bk, bf, (u64)q.top_k - 1, one);
+            if (n < 0) {
+                if (small || (q.top_k && upto <= CAP)) n = gather([&](float x, int) { return bin(x) <= min(bk, NB - 2); });
+                else if (q.top_k && bk < NB - 1) last = resolve(bk, bf, (u64)q.top_k - 1, one);
+            }
         }
         u64 before, total;
         float xv = top;
@@ -686,7 +709,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleP p) {
 
 // ------------------------------------------------------------------------------------------------ few categories
 // L lanes per row (a power of two), a lane per category.  A lane finds what precedes it in the order by looking at every other one.
-// 16384 rows of 60, top-p: 44 us, against 46 by a wave per row; of 24: 14.5 against 35.
+// 16384 rows of 60, top-p: 32 us, against 46 by a workgroup of one wave for each (44 with exchanges through LDS instead of v_readlane);
+// of 24: 14.5 against 35.
 template <class E, int L>
 __global__ __launch_bounds__(256) void sample_few_kernel(SampleP p) {
     const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
@@ -710,8 +734,8 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleP p) {
     u64 weight = 0;
     if (__any(q.top_k != 0 || q.top_p < 1.f)) {
         for (int i = 0; i < L; ++i) {
-            const float xi = __shfl(x, i, L);
-            const u64 wi = (u64)__shfl((long long)w, i, L);
+            const float xi = L == 64 ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)) : __shfl(x, i, L);
+            const u64 wi = L == 64 ? lane_u64(w, i) : (u64)__shfl((long long)w, i, L);
             if (xi > x || (xi == x && i < j)) {
                 ++before;
                 weight += wi;

@@ -92,6 +92,23 @@ def test_many_long_rows(rows, V, dtype):
         torch.testing.assert_close(tok[keep], want, rtol=0, atol=0)
 
 
+@pytest.mark.parametrize("V", [1000, 4099, 20001])
+def test_top_k_where_the_largest_lie_together(V):
+    """Sorted rows, the largest in one stretch, fewer finite logits than top_k, and a +inf among them, for top_k around half the threads."""
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    lg = _logits(gen, 6, V, "f32")
+    lg[0] = lg[0].sort(descending=True).values
+    lg[1] = lg[1].sort().values
+    lg[2, 100:400] += 9.0
+    lg[3] = -float("inf")
+    lg[3, 5::V // 9] = 1.0
+    lg[4, 77] = float("inf")
+    lg[4, 900] = float("inf")
+    for k in (2, 20, 32, 33, 128, 129, 512, 513):
+        for p in (1.0, 0.9):
+            _check(lg, torch.rand(6, device="cuda", generator=gen), top_k=k, top_p=p)
+
+
 def test_a_lead_that_ends_where_top_k_does():
     """top-k's last element, the lead's last element and min-p's limit in one bin, in rows that start off a 16-byte boundary."""
     gen = torch.Generator(device="cuda").manual_seed(9)
