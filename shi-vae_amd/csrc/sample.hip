@@ -592,6 +592,9 @@ struct Sampler {
         // 2. all that top-k keeps, or a small row, into the list
         int n = -1;  // elements in the list, if it holds all candidates
         if (q.top_k || q.top_p < 1.f) {
+            // Sorting a list of all that is kept, or the bin of the last one and then (top-p) the row's weights once more?  us: 1 x 32768, top-k 1000
+            // 45 / 30, with top-p 0.5 35 / 46; 64 x 8000 51 / 23, with top-p 37 / 32; 4096 x 2048, top-k 400 90 / 38, with top-p 0.9 74 / 57.
+            const u64 longest = min(CAP, q.top_p < 1.f ? 2 * NT : max(128, NT / 2));
             int bk = NB - 2;
             u64 bf = 0, total = 0, upto = 0;
             const bool small = V <= 128;  // (ranks by counting; longer rows are cheaper by the histogram: 4096 x 512, top-p, 24 us against 60)
@@ -613,7 +616,7 @@ struct Sampler {
                 upto = bk < NB - 1 ? bf + s.hist[bk] : total;
             }
             if (n < 0) {
-                if (small || (q.top_k && upto <= CAP)) n = gather([&](float x, int) { return bin(x) <= min(bk, NB - 2); });
+                if (small || (q.top_k && upto <= longest)) n = gather([&](float x, int) { return bin(x) <= min(bk, NB - 2); });
                 else if (q.top_k && bk < NB - 1) last = resolve(bk, bf, (u64)q.top_k - 1, one);
             }
         }
