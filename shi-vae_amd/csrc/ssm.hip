@@ -184,6 +184,13 @@ __device__ __forceinline__ float swap16_add(float x, float y) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// The sums over the four state groups of four rows' parts, row i in lane row i.  The swaps read a VGPR two wait states after a vector
+// instruction wrote it at the earliest, and the compiler does not see the last instruction of row_dot's assembly (S >= 4).
+template <int S>
+__device__ __forceinline__ float sum_groups(float (&v)[4]) {
+    if constexpr (S >= 4) asm("s_nop 1" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+    return swap16_add(swap32_add(v[0], v[2]), swap32_add(v[1], v[3]));
+}
 template <int N, class F>
 __device__ __forceinline__ void unroll(F f) {  // f(0), f(1), ... with the number as a constant
     [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
@@ -315,7 +322,7 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
                 for (int j = 0; j < S; ++j) h[j] = fmaf(__builtin_amdgcn_exp2f(x[r].x * A2[j]), h[j], row_of<r>(vB[j]) * x[r].y);
                 if constexpr (!FIRST) acc[i] = row_dot<r>(vC, h);
             });
-            if constexpr (!FIRST) v[k] = fmaf(Dp, ku[k], swap16_add(swap32_add(acc[0], acc[2]), swap32_add(acc[1], acc[3])));
+            if constexpr (!FIRST) v[k] = fmaf(Dp, ku[k], sum_groups<S>(acc));
             pz[k] = kz[k];
         });
         // The next tile is taken over in front of this one's stores: stores and loads share a counter that is waited for in order.
@@ -732,7 +739,7 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
                     }
                     acc[i] = row_dot<r>(vC, h[r]);
                 });
-                const float y = swap16_add(swap32_add(acc[0], acc[2]), swap32_add(acc[1], acc[3]));
+                const float y = sum_groups<S>(acc);
                 sum3[0][k][lane] = MANY && pass ? sum3[0][k][lane] + y : y;
                 __builtin_amdgcn_sched_barrier(0);  // (or the scheduler starts all rows at once and runs out of registers)
             });
@@ -774,7 +781,7 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
                 rs[i] = gs;
                 if constexpr (i == 0) __builtin_amdgcn_sched_barrier(0);
                 if constexpr (i == 0) {
-                    const float gb = swap16_add(swap32_add(rb[0], rb[2]), swap32_add(rb[1], rb[3]));
+                    const float gb = sum_groups<S>(rb);
                     const float gs4 = swap16_add(swap32_add(rs[0], rs[2]), swap32_add(rs[1], rs[3]));
                     sum3[1][r / 4][lane] = MANY && pass ? sum3[1][r / 4][lane] + gb : gb;
                     sum3[2][r / 4][lane] = MANY && pass ? sum3[2][r / 4][lane] + gs4 : gs4;
