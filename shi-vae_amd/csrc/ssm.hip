@@ -45,8 +45,12 @@ __device__ __forceinline__ int ssm_len(const SsmP& p, int b) {
     return n < 0 ? 0 : (n < p.a.T ? n : p.a.T);
 }
 
-// A log2(e), finite: an A of -inf (no memory) has to give exp(0 A) = 1 behind a sequence's end, and 0 where a step is positive.
-__device__ __forceinline__ float scale_A(float A) { return fminf(fmaxf(A * kLog2e, -3.4e38f), 3.4e38f); }
+// A log2(e), infinities made finite: an A of -inf (no memory) has to give exp(0 A) = 1 behind a sequence's end, and 0 where a step is
+// positive.  A NaN stays one (comparisons, since fminf and fmaxf return the other operand).
+__device__ __forceinline__ float scale_A(float A) {
+    const float v = A * kLog2e;
+    return v < -3.4e38f ? -3.4e38f : (v > 3.4e38f ? 3.4e38f : v);
+}
 
 // One workgroup's place: piece, sequence, group, and this lane's channel.
 struct Place {
@@ -211,6 +215,7 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
     if (!__any(q.ok)) return;
     const int n = ssm_len(p, q.b), t0 = q.piece * p.plen, t1 = min(a.T, t0 + p.plen), tn = min(t1, n);
     const int64_t state0 = ((int64_t)q.b * a.N + g4 * S) * a.D + q.d, statep = (int64_t)a.B * a.N * a.D;
+    const int pieces = (n + p.plen - 1) / p.plen;  // that hold rows of the sequence
 
     float h[S], A2[S];
 #pragma unroll
@@ -219,11 +224,13 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
         const int64_t o = state0 + (int64_t)j * a.D;
         A2[j] = live ? scale_A(a.A[(int64_t)(g4 * S + j) * a.D + q.d]) : 0.f;
         h[j] = live && q.piece == 0 && a.state ? a.state[o] : 0.f;
-        if (!FIRST && live)
-            for (int c = 0; c < q.piece; ++c) {
+        if (!FIRST && live && q.piece) {
+            h[j] = p.hend[o];
+            for (int c = 1; c < min(q.piece, pieces); ++c) {
                 const float sum = p.ssum[((int64_t)c * a.B + q.b) * a.D + q.d];
                 h[j] = fmaf(__builtin_amdgcn_exp2f(A2[j] * sum), h[j], p.hend[c * statep + o]);
             }
+        }
     }
     const float bias = a.dt_bias ? a.dt_bias[q.d] : 0.f, Dp = (!FIRST && a.Dp) ? a.Dp[q.d] : 0.f;
     const unsigned le = q.lo * (unsigned)sizeof(E);
@@ -412,12 +419,12 @@ __global__ __launch_bounds__(256) void ssm_token_kernel(SsmP p, int nvec) {
 
 // Where the adjoint of a piece's last state comes from: the gradient of state_out for the last piece, otherwise what the pieces behind
 // it hand down (prod_t exp(s_t A) = exp(A sum_t s_t), as in the forward pass).
-__device__ __forceinline__ float piece_adjoint(const SsmP& p, const Place& q, int s, float A2) {
+__device__ __forceinline__ float piece_adjoint(const SsmP& p, const Place& q, int n, int s, float A2) {
     const shivae_ssm_args& a = p.a;
     const int64_t o = ((int64_t)q.b * a.N + s) * a.D + q.d;
     if (q.piece == p.np - 1) return a.dstate_out ? a.dstate_out[o] : 0.f;
-    float v = 0.f;
-    for (int c = p.np - 1; c > q.piece; --c)
+    float v = p.hend[(int64_t)(p.np - 1) * a.B * a.N * a.D + o];
+    for (int c = min(p.np - 1, (n + p.plen - 1) / p.plen) - 1; c > q.piece; --c)  // (pieces behind the sequence's end hand on what they get)
         v = fmaf(__builtin_amdgcn_exp2f(A2 * p.ssum[((int64_t)c * a.B + q.b) * a.D + q.d]), v, p.hend[(int64_t)c * a.B * a.N * a.D + o]);
     return v;
 }
@@ -520,11 +527,18 @@ __global__ __launch_bounds__(256) void ssm_bwd_first_kernel(SsmP p) {
         float2 x[TT];
 #pragma unroll
         for (int r = 0; r < TT; ++r) x[r] = row[r][lane & 15];
-        unroll<TT>([&](auto I) {
-            constexpr int r = TT - 1 - I;
+        auto run = [&](auto whole) {
+            unroll<TT>([&](auto I) {
+                constexpr int r = TT - 1 - I;
 #pragma unroll
-            for (int j = 0; j < S; ++j) ag[j] = __builtin_amdgcn_exp2f(x[r].x * A2[j]) * (ag[j] + row_of<r>(vC[j]) * x[r].y);
-        });
+                for (int j = 0; j < S; ++j) {
+                    const float v = __builtin_amdgcn_exp2f(x[r].x * A2[j]) * (ag[j] + row_of<r>(vC[j]) * x[r].y);
+                    ag[j] = whole || r < left ? v : ag[j];  // (behind the sequence's end exp(0 A) is no 1 where A is NaN)
+                }
+            });
+        };
+        if (left >= TT) run(std::true_type{});
+        else run(std::false_type{});
     }
 #pragma unroll
     for (int j = 0; j < S; ++j)
@@ -637,7 +651,7 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
             const int s = k * P + g4 * S + j;
             const bool live = q.ok && s < a.N;
             A2[j] = live ? scale_A(a.A[(int64_t)s * a.D + q.d]) : 0.f;
-            ag[j] = live ? piece_adjoint(p, q, s, A2[j]) : 0.f;
+            ag[j] = live ? piece_adjoint(p, q, n, s, A2[j]) : 0.f;
             dA[j] = 0.f;
             if (MANY) {
                 float* o = kept + (int64_t)k * 3 * S * 256 + threadIdx.x;
@@ -743,6 +757,13 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
                 sum3[0][k][lane] = MANY && pass ? sum3[0][k][lane] + y : y;
                 __builtin_amdgcn_sched_barrier(0);  // (or the scheduler starts all rows at once and runs out of registers)
             });
+            if (left < TT)  // (behind the sequence's end exp(0 A) is no 1 where A is NaN)
+                unroll<TT>([&](auto R) {
+                    constexpr int r = R;
+                    if (r >= left)
+#pragma unroll
+                        for (int j = 0; j < S; ++j) e[r][j] = 1.f;
+                });
             // Everything that the way back takes from LDS and from B and C is taken again: kept from the way there it would be 10 S + 32
             // registers that are not free.
             asm volatile("" ::: "memory");
