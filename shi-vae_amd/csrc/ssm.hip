@@ -52,6 +52,13 @@ __device__ __forceinline__ float scale_A(float A) {
     return v < -3.4e38f ? -3.4e38f : (v > 3.4e38f ? 3.4e38f : v);
 }
 
+// 2^x v + add, where 2^x alone may leave the range of fp32: x is the sum of a piece's log2 decays, and decays that grow (s A > 0) take a
+// state of 0, or a small one, through a piece without ever leaving the range.
+__device__ __forceinline__ float decay_add(float x, float v, float add) {
+    const float k = fabsf(x) <= 126.f ? 0.f : rintf(fminf(fmaxf(x, -1e4f), 1e4f)), f = (x > 1e4f ? 1e4f : x) - k;
+    return fmaf(__builtin_amdgcn_exp2f(f), __builtin_amdgcn_ldexpf(v, (int)k), add);
+}
+
 // One workgroup's place: piece, sequence, group, and this lane's channel.
 struct Place {
     int piece, b, g, tile;
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
             h[j] = p.hend[o];
             for (int c = 1; c < min(q.piece, pieces); ++c) {
                 const float sum = p.ssum[((int64_t)c * a.B + q.b) * a.D + q.d];
-                h[j] = fmaf(__builtin_amdgcn_exp2f(A2[j] * sum), h[j], p.hend[c * statep + o]);
+                h[j] = decay_add(A2[j] * sum, h[j], p.hend[c * statep + o]);
             }
         }
     }
@@ -425,7 +432,7 @@ __device__ __forceinline__ float piece_adjoint(const SsmP& p, const Place& q, in
     if (q.piece == p.np - 1) return a.dstate_out ? a.dstate_out[o] : 0.f;
     float v = p.hend[(int64_t)(p.np - 1) * a.B * a.N * a.D + o];
     for (int c = min(p.np - 1, (n + p.plen - 1) / p.plen) - 1; c > q.piece; --c)  // (pieces behind the sequence's end hand on what they get)
-        v = fmaf(__builtin_amdgcn_exp2f(A2 * p.ssum[((int64_t)c * a.B + q.b) * a.D + q.d]), v, p.hend[(int64_t)c * a.B * a.N * a.D + o]);
+        v = decay_add(A2 * p.ssum[((int64_t)c * a.B + q.b) * a.D + q.d], v, p.hend[(int64_t)c * a.B * a.N * a.D + o]);
     return v;
 }
 

@@ -4,7 +4,9 @@ import numpy as np
 import pytest
 import torch
 
+import _seq_ref as ref
 import shivae_amd
+from test_gpu_seq_ops import _near
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +87,53 @@ def test_nan_everywhere_else_is_seen():
         y, last = shivae_amd.selective_scan(**w, return_state=True)
         assert torch.isnan(y[50, 1, 4]), k
         assert torch.isnan(last[1, 3, 4]) == (k in ("u", "dt", "B", "dt_bias", "initial_state")), k
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("B", [1, 260])
+def test_growing_decays_over_a_state_of_zero(B, sign):
+    """Decays whose product over a piece of the time axis overflows, while state and adjoint there are 0: the pieces (one sequence) give
+    what the unsplit scan (260 sequences fill the card) and the formula give.  A > 0 with positive steps, and A < 0 with negative."""
+    T, D, Ns = 200, 40, 16
+    v, dy, _ = _inputs(T, B, D, Ns)
+    for k in ("D", "z", "dt_bias", "initial_state"):
+        v[k] = None
+    v["A"] = -v["A"] * sign
+    grow = torch.full_like(v["dt"], 3.0 * sign)
+    calm = 0.02 * v["dt"].abs() * sign
+    # forward: growth in rows 0..129, in front of all input (exp(3 * 0.2) a row at least: past 2^128 within 150 rows)
+    v["dt"] = torch.where(torch.arange(T, device="cuda")[:, None, None] < 130, grow, calm)
+    v["u"][:130] = 0
+    a = {k: None if t is None else t.double().cpu().numpy() for k, t in v.items()}
+    want, scale = ref.scan(a["u"], a["dt"], a["A"], a["B"], a["C"], None, None, None, None, None, False)
+    assert float(np.abs(a["A"]).max()) * 3 * 64 > 88.8  # past the largest fp32 within a piece
+    y, last = shivae_amd.selective_scan(v["u"], v["dt"], v["A"], v["B"], v["C"], softplus=False, return_state=True)
+    _near(y, want["y"], scale["y"], 3 * T + 96, "y")
+    _near(last, want["last"], scale["last"], 3 * T + 96, "state")
+    # backward: growth in rows 70..199, behind all gradient
+    v["dt"] = torch.where(torch.arange(T, device="cuda")[:, None, None] < 70, calm, grow)
+    v["u"][:] = 0
+    dy[70:] = 0
+    a = {k: None if t is None else t.double().cpu().numpy() for k, t in v.items()}
+    want, scale = ref.scan(a["u"], a["dt"], a["A"], a["B"], a["C"], None, None, None, None, None, False, dy.double().cpu().numpy())
+    leaves = [v[k].clone().requires_grad_(True) for k in ("u", "dt", "A", "B", "C")]
+    y = shivae_amd.selective_scan(*leaves, softplus=False)
+    for k, g in zip(("u", "dt", "A", "B", "C"), torch.autograd.grad(y, leaves, dy)):
+        _near(g, want[k], scale[k], 2 * (3 * T + 96) + 8 + np.log2(T * B) + T, "d" + k)
+
+
+@pytest.mark.parametrize("x", [-240, 240])
+def test_states_far_out_of_the_ordinary(x):
+    """A large state that decays, and a small one that grows, by 2^x over the second of three pieces: 2^x is out of the range of fp32, the
+    states are not.  The exponent is off by a unit for log2(e) and one for A log2(e), relative to |x| log(2) = sum |s A|."""
+    T, D, Ns = 192, 8, 4
+    rows = torch.arange(T, device="cuda")[:, None, None]
+    u, one = torch.zeros(T, 1, D, device="cuda"), torch.ones(T, 1, 1, Ns, device="cuda")
+    dt = torch.where((rows >= 64) & (rows < 128), 1.0, 0.0).expand(T, 1, D).contiguous()
+    A = torch.full((Ns, D), x * np.log(2.0) / 64, device="cuda")
+    s0 = torch.full((1, Ns, D), 2.0 ** (-x // 2), device="cuda")
+    y, last = shivae_amd.selective_scan(u, dt, A, one, one, softplus=False, initial_state=s0, return_state=True)
+    total = 64 * A.double().cpu().numpy()
+    want = s0.double().cpu().numpy() * np.exp(total)
+    _near(last, want, want, 3 * T + 96 + 2 * np.abs(total).max(), "state")
+    _near(y[128:], np.broadcast_to(want.sum(1), (64, 1, D)), want.sum(), 3 * T + 96 + 2 * np.abs(total).max(), "y")
