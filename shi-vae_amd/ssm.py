@@ -9,10 +9,12 @@ the arithmetic: every result is rounded once, where it is stored.
 ``lengths`` ([B], int32 or int64, on the device) gives the number of rows of each sequence (clamped to 0..T); rows behind
 it are not read, outputs and gradients are 0 there, and the state that comes out is the one behind the last row.
 
-All calls enqueue on the current stream of the tensors' device and do not synchronise.  There is no CPU fallback."""
+All calls enqueue on the current stream of the tensors' device and do not synchronise.  There is no CPU fallback.  The sequence forms
+have a first derivative in reverse mode; dual tensors of forward mode are refused."""
 from ctypes import byref
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version  # a state written in place that a backward pass still needs is an error there
 
@@ -88,7 +90,15 @@ def _call(device, f, *args):
         N.check(rc)
 
 
+def _no_tangents(*tensors):
+    if forward_ad._current_level >= 0:  # (inside of a dual_level: otherwise no tensor has a tangent)
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the sequence operators and the sampler have no forward-mode derivative: unpack the dual tensor, or use the backward pass")
+
+
 def _wants_grad(*tensors):
+    _no_tangents(*tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -147,6 +157,7 @@ class _CausalConv(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dlast):
         x, weight, bias, state, lengths = ctx.saved_tensors
+        _no_tangents(dy, dlast)
         dy = torch.zeros_like(x) if dy is None else _rows(dy)
         dlast = None if dlast is None else dlast.contiguous()
         dx, dw = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty_like(weight)
@@ -250,6 +261,7 @@ class _SelectiveScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dlast):
         u, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, ckpt = ctx.saved_tensors
+        _no_tangents(dy, dlast)
         dy = torch.zeros_like(u) if dy is None else _rows(dy)
         dlast = None if dlast is None else dlast.contiguous()
 

@@ -1,0 +1,46 @@
+"""Derivatives that the sequence operators and the sampler do not have are refused, not dropped."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import shivae_amd
+
+pytestmark = pytest.mark.gpu
+
+
+def _calls():
+    gen = torch.Generator(device="cuda").manual_seed(0)
+
+    def rn(*shape):
+        return torch.randn(*shape, device="cuda", generator=gen)
+
+    T, B, D, Ns = 5, 2, 8, 4
+    x, w, b, cs = rn(T, B, D), rn(4, D), rn(D), rn(3, B, D)
+    scan = dict(u=rn(T, B, D), dt=rn(T, B, D), A=-rn(Ns, D).abs(), B=rn(T, B, 1, Ns), C=rn(T, B, 1, Ns), D=rn(D), z=rn(T, B, D), dt_bias=rn(D))
+    step = {k: t[0] if t.dim() > 2 else t for k, t in scan.items()}
+    ss = rn(B, Ns, D)
+    return [(shivae_amd.causal_conv, dict(x=x, weight=w, bias=b, initial_state=cs)),
+            (shivae_amd.causal_conv_step, dict(x=x[0], weight=w, bias=b, state=cs)),
+            (shivae_amd.selective_scan, dict(**scan, initial_state=ss)),
+            (shivae_amd.selective_scan_step, dict(**step, state=ss))]
+
+
+def test_forward_mode_is_refused():
+    for f, kw in _calls():
+        for k, t in kw.items():
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                        f(**{**kw, k: dual})
+                f(**kw)  # (no tangent: the call is as ever)
+
+
+def test_forward_mode_through_a_backward_pass_is_refused():
+    for f, kw in _calls()[::2]:
+        leaf = next(iter(kw.values())).requires_grad_(True)
+        y = f(**kw)
+        with forward_ad.dual_level():
+            dy = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, dy)
