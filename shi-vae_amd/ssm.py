@@ -10,12 +10,11 @@ the arithmetic: every result is rounded once, where it is stored.
 it are not read, outputs and gradients are 0 there, and the state that comes out is the one behind the last row.
 
 All calls enqueue on the current stream of the tensors' device and do not synchronise.  There is no CPU fallback.  The sequence forms
-have a first derivative in reverse mode; dual tensors of forward mode are refused."""
+have a first derivative in reverse mode; a derivative of it, and dual tensors of forward mode, are refused."""
 from ctypes import byref
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version  # a state written in place that a backward pass still needs is an error there
 
 from . import _native as N
@@ -122,6 +121,23 @@ def _step_state(state, state_out):
     return state_out
 
 
+class _Recorded(torch.autograd.Function):
+    """The result of a backward pass that is itself recorded (create_graph), as a function of all that it depends on: a derivative that
+    passes through it raises."""
+    @staticmethod
+    def forward(ctx, grads, *depends_on):
+        return grads()
+
+    @staticmethod
+    def backward(ctx, *g):
+        raise RuntimeError("the sequence operators have no second derivative")
+
+
+def _first_derivative(grads, *depends_on):
+    _no_tangents(*depends_on)
+    return _Recorded.apply(grads, *depends_on) if torch.is_grad_enabled() else grads()
+
+
 def _no_backward(*tensors):
     if _wants_grad(*tensors):
         raise RuntimeError("the single-token steps have no backward pass: call them under torch.no_grad(), or use the sequence form with one row")
@@ -145,6 +161,19 @@ def _conv_forward(x, weight, bias, state, lengths, silu, want_state):
     return y, last
 
 
+def _conv_backward(x, weight, bias, state, lengths, silu, dy, dlast):
+    dy = torch.zeros_like(x) if dy is None else _rows(dy)
+    dlast = None if dlast is None else dlast.contiguous()
+    dx, dw = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty_like(weight)
+    db = None if bias is None else torch.empty_like(bias)
+    ds = None if state is None else torch.empty_like(state)
+    args = _conv_args(x, weight, bias, state, lengths, silu, None, None, dy, dlast, dx, dw, db, ds)
+    L = N.lib()
+    ws = torch.empty(L.shivae_causal_conv_bwd_ws(byref(args)), dtype=torch.uint8, device=x.device)
+    _call(x.device, L.shivae_causal_conv_bwd, byref(args), ws.data_ptr(), ws.numel())
+    return dx, dw, db, ds
+
+
 class _CausalConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, lengths, silu, want_state):
@@ -154,20 +183,10 @@ class _CausalConv(torch.autograd.Function):
         return _conv_forward(x, weight, bias, state, lengths, silu, want_state)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dlast):
         x, weight, bias, state, lengths = ctx.saved_tensors
-        _no_tangents(dy, dlast)
-        dy = torch.zeros_like(x) if dy is None else _rows(dy)
-        dlast = None if dlast is None else dlast.contiguous()
-        dx, dw = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty_like(weight)
-        db = None if bias is None else torch.empty_like(bias)
-        ds = None if state is None else torch.empty_like(state)
-        args = _conv_args(x, weight, bias, state, lengths, ctx.silu, None, None, dy, dlast, dx, dw, db, ds)
-        L = N.lib()
-        ws = torch.empty(L.shivae_causal_conv_bwd_ws(byref(args)), dtype=torch.uint8, device=x.device)
-        _call(x.device, L.shivae_causal_conv_bwd, byref(args), ws.data_ptr(), ws.numel())
-        return dx, dw, db, ds, None, None, None
+        grads = _first_derivative(lambda: _conv_backward(x, weight, bias, state, lengths, ctx.silu, dy, dlast), x, weight, bias, state, dy, dlast)
+        return (*grads, None, None, None)
 
 
 def _conv_silu(activation):
@@ -248,6 +267,22 @@ def _scan_forward(u, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, softplus, wan
     return y, last, ckpt
 
 
+def _scan_backward(u, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, ckpt, softplus, dy, dlast):
+    dy = torch.zeros_like(u) if dy is None else _rows(dy)
+    dlast = None if dlast is None else dlast.contiguous()
+
+    def like(t):
+        return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+    du, ddt, dz, dB, dC, dA, dD, db, ds = (like(t) for t in (u, dt, z, Bm, Cm, A, D, dt_bias, state))
+    args = _scan_args(u, dt, z, Bm, Cm, A, D, dt_bias, state, lengths, softplus, None, None, ckpt, dy, dlast, du, ddt, dz, dB, dC, dA, dD,
+                      db, ds)
+    L = N.lib()
+    ws = torch.empty(L.shivae_selective_scan_bwd_ws(byref(args)), dtype=torch.uint8, device=u.device)
+    _call(u.device, L.shivae_selective_scan_bwd, byref(args), ws.data_ptr(), ws.numel())
+    return du, ddt, dA, dB, dC, dD, dz, db, ds
+
+
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, softplus, want_state):
@@ -258,23 +293,10 @@ class _SelectiveScan(torch.autograd.Function):
         return y, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dlast):
-        u, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, ckpt = ctx.saved_tensors
-        _no_tangents(dy, dlast)
-        dy = torch.zeros_like(u) if dy is None else _rows(dy)
-        dlast = None if dlast is None else dlast.contiguous()
-
-        def like(t):
-            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-        du, ddt, dz, dB, dC, dA, dD, db, ds = (like(t) for t in (u, dt, z, Bm, Cm, A, D, dt_bias, state))
-        args = _scan_args(u, dt, z, Bm, Cm, A, D, dt_bias, state, lengths, ctx.softplus, None, None, ckpt, dy, dlast, du, ddt, dz, dB, dC,
-                          dA, dD, db, ds)
-        L = N.lib()
-        ws = torch.empty(L.shivae_selective_scan_bwd_ws(byref(args)), dtype=torch.uint8, device=u.device)
-        _call(u.device, L.shivae_selective_scan_bwd, byref(args), ws.data_ptr(), ws.numel())
-        return du, ddt, dA, dB, dC, dD, dz, db, ds, None, None, None
+        saved = ctx.saved_tensors
+        grads = _first_derivative(lambda: _scan_backward(*saved, ctx.softplus, dy, dlast), *saved[:9], dy, dlast)
+        return (*grads, None, None, None)
 
 
 def _scan_inputs(u, dt, A, B, C_, D, z, dt_bias):

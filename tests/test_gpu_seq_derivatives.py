@@ -44,3 +44,21 @@ def test_forward_mode_through_a_backward_pass_is_refused():
             dy = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(y, leaf, dy)
+
+
+def test_second_derivatives_are_refused():
+    """A recorded gradient may be used; what differentiates it raises, also where the gradient came from a constant or reaches the leaf by
+    another path too."""
+    for f, kw in _calls()[::2]:
+        for k in kw:
+            leaves = {**kw, k: kw[k].detach().clone().requires_grad_(True)}
+            for loss in (torch.Tensor.sum, lambda y: y.square().sum()):
+                y = f(**leaves)
+                want, = torch.autograd.grad(loss(y), leaves[k], retain_graph=True)
+                g, = torch.autograd.grad(loss(y), leaves[k], create_graph=True)
+                assert torch.equal(g, want)
+                total = loss(y) + g.square().sum()
+                with pytest.raises(RuntimeError, match="second derivative"):
+                    torch.autograd.grad(total, leaves[k], retain_graph=True)
+                with pytest.raises(RuntimeError, match="second derivative"):
+                    total.backward()
