@@ -5,7 +5,7 @@ from ctypes import byref
 import torch
 
 from . import _native as N
-from .ssm import _DTYPES, _call
+from .ssm import _DTYPES, _call, _wants_grad
 
 MAX_CATEGORIES = 1048512  # SHIVAE_SAMPLE_MAX
 
@@ -40,11 +40,14 @@ def sample_categories(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     everything.  Sums are exact (weights are held to 2^-43 of the largest), so the result does not depend on scheduling.
 
     Returns int64 indices [...], or (indices, log-probability of the index among the kept [...] float32); the log-probability
-    is 0 for temperature 0 and -inf where the index is -1."""
+    is 0 for temperature 0 and -inf where the index is -1.  It has no derivative: with logits or a temperature that require one the call
+    is refused, under torch.no_grad() or with detached tensors it is not."""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES:
         raise TypeError("logits must be a float32, bfloat16 or float16 tensor")
     if logits.dim() < 1 or logits.numel() == 0:
         raise ValueError("logits of shape %s have nothing to draw from" % (tuple(logits.shape),))
+    if return_logprob and _wants_grad(logits, temperature if isinstance(temperature, torch.Tensor) else None):
+        raise RuntimeError("the log-probability has no derivative: call under torch.no_grad(), or detach logits and temperature")
     V = logits.shape[-1]
     if V > MAX_CATEGORIES:
         raise ValueError("%d categories, up to %d are supported" % (V, MAX_CATEGORIES))

@@ -62,3 +62,21 @@ def test_second_derivatives_are_refused():
                     torch.autograd.grad(total, leaves[k], retain_graph=True)
                 with pytest.raises(RuntimeError, match="second derivative"):
                     total.backward()
+
+
+def test_the_log_probability_is_not_differentiable():
+    """It is refused where a gradient would be lost; indices have none, as those of argmax."""
+    lg, u, t = torch.randn(3, 50, device="cuda"), torch.rand(3, device="cuda"), torch.ones(3, device="cuda")
+    f = shivae_amd.sample_categories
+    want, logp = f(lg, u, t, return_logprob=True)
+    for kw in (dict(logits=lg.clone().requires_grad_(True), temperature=t), dict(logits=lg, temperature=t.clone().requires_grad_(True))):
+        with pytest.raises(RuntimeError, match="no derivative"):
+            f(u=u, return_logprob=True, **kw)
+        assert torch.equal(f(u=u, **kw), want)
+        with torch.no_grad():
+            assert torch.equal(f(u=u, return_logprob=True, **kw)[1], logp)
+        detached = {k: v.detach() for k, v in kw.items()}
+        assert torch.equal(f(u=u, return_logprob=True, **detached)[1], logp)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            f(forward_ad.make_dual(lg, torch.ones_like(lg)), u, t, return_logprob=True)
