@@ -311,7 +311,9 @@ int shivae_causal_conv_fwd(const shivae_conv_args* args, shivae_stream stream) {
     ConvP p{a, ceil_div(a.D, v), conv_run(a, v, false), 0, nullptr};
     p.nrun = ceil_div(a.T, p.run);
     SV_REQUIRE(!a.state || a.state != a.state_out || p.nrun == 1, "causal_conv_fwd: the state can be updated in place for up to %d time steps only", p.run);
-    const dim3 grid((unsigned)(((int64_t)a.B * p.nvec + 255) / 256), p.nrun);
+    const int64_t blocks = ((int64_t)a.B * p.nvec + 255) / 256;
+    SV_REQUIRE(grid_fits(blocks, 256), "causal_conv_fwd: B * D is too large (%d sequences of %d channel groups)", a.B, p.nvec);
+    const dim3 grid((unsigned)blocks, p.nrun);
     SV_BY_DTYPE(a.dtype, {
         if (v > 1) launch_conv<E, 16 / (int)sizeof(E)>(false, p, grid, static_cast<hipStream_t>(stream));
         else launch_conv<E, 1>(false, p, grid, static_cast<hipStream_t>(stream));
@@ -333,13 +335,15 @@ int shivae_causal_conv_bwd(const shivae_conv_args* args, void* ws_dev, size_t ws
     SV_REQUIRE(a.dy && a.dx && a.dweight, "causal_conv_bwd: dy, dx and dweight are required");
     SV_REQUIRE(!a.state || a.dstate, "causal_conv_bwd: a state that came in needs a buffer for its gradient");
     SV_REQUIRE(a.dbias || !a.bias, "causal_conv_bwd: a bias needs a buffer for its gradient");
-    const size_t need = shivae_causal_conv_bwd_ws(args);
-    SV_REQUIRE(ws_dev && ws_bytes >= need, "causal_conv_bwd: workspace of %zu bytes is smaller than %zu", ws_bytes, need);
-    SV_REQUIRE(aligned_to(ws_dev, 16), "causal_conv_bwd: the workspace must be 16-byte aligned");
     const int v = conv_vec(a, true);
     ConvP p{a, ceil_div(a.D, v), conv_run(a, v, true), 0, static_cast<float*>(ws_dev)};
     p.nrun = ceil_div(a.T, p.run);
-    const dim3 grid((unsigned)(((int64_t)a.B * p.nvec + 255) / 256), p.nrun);
+    const int64_t blocks = ((int64_t)a.B * p.nvec + 255) / 256;
+    SV_REQUIRE(grid_fits(blocks, 256), "causal_conv_bwd: B * D is too large (%d sequences of %d channel groups)", a.B, p.nvec);
+    const size_t need = shivae_causal_conv_bwd_ws(args);
+    SV_REQUIRE(ws_dev && ws_bytes >= need, "causal_conv_bwd: workspace of %zu bytes is smaller than %zu", ws_bytes, need);
+    SV_REQUIRE(aligned_to(ws_dev, 16), "causal_conv_bwd: the workspace must be 16-byte aligned");
+    const dim3 grid((unsigned)blocks, p.nrun);
     hipStream_t s = static_cast<hipStream_t>(stream);
     SV_BY_DTYPE(a.dtype, {
         if (v > 1) launch_conv<E, 16 / (int)sizeof(E)>(true, p, grid, s);

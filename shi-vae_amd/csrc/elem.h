@@ -41,6 +41,8 @@ __device__ __forceinline__ float seq_softplus(float v) {
         }                                          \
     } while (0)
 
+// A launch has fewer than 2^32 threads along an axis (hipModuleLaunchKernel).
+static inline bool grid_fits(int64_t blocks, int threads) { return blocks < ((int64_t)1 << 32) / threads; }
 static inline int elem_bytes(int dtype) { return dtype == SHIVAE_F32 ? 4 : 2; }
 static inline bool aligned_to(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 

@@ -18,6 +18,8 @@
 // bin too full for the list (runs of equal values) is resolved by four 8-bit digits of the key instead.  Bound by the row's reads
 // for few kept elements (the row stays in L2 between the passes) and by vector instructions for many: about 25 for an exponential in 64
 // bits, 100 per category in all with top-p.
+#include <algorithm>
+
 #include "common.h"
 #include "elem.h"
 
@@ -777,7 +779,7 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleP p) {
 }
 
 template <class E>
-static void launch_sample(const SampleP& p, hipStream_t s) {
+static void launch_sample(const SampleP& p, int64_t all_rows, hipStream_t s) {
     const int V = p.a.V;
     if (V <= 64) {
         const int L = V <= 2 ? 2 : V <= 4 ? 4 : V <= 8 ? 8 : V <= 16 ? 16 : V <= 32 ? 32 : 64;
@@ -795,8 +797,8 @@ static void launch_sample(const SampleP& p, hipStream_t s) {
     // 256 x 16384 with 256 / 1024 threads 36 / 31.7, 256 x 8192 24.0 / 25.1, 512 x 32768 77 / 89, 1024 x 32768 119 / 176.  (A row's sums of 64
     // vectors have to fit the histogram, so that the longest rows take 1024 threads however many they are.)
     const dim3 grid((unsigned)p.a.rows);
-    if (V <= 512 || (V <= 4096 && p.a.rows >= 2048)) hipLaunchKernelGGL((sample_kernel<E, 64, 512, 256>), grid, dim3(64), 0, s, p);
-    else if (V <= 8192 || (V <= 262144 && p.a.rows >= 512)) hipLaunchKernelGGL((sample_kernel<E, 256, 2048, 2048>), grid, dim3(256), 0, s, p);
+    if (V <= 512 || (V <= 4096 && all_rows >= 2048)) hipLaunchKernelGGL((sample_kernel<E, 64, 512, 256>), grid, dim3(64), 0, s, p);
+    else if (V <= 8192 || (V <= 262144 && all_rows >= 512)) hipLaunchKernelGGL((sample_kernel<E, 256, 2048, 2048>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((sample_kernel<E, 1024, 4096, 4096>), grid, dim3(1024), 0, s, p);
 }
 
@@ -811,8 +813,21 @@ extern "C" int shivae_sample_categories(const shivae_sample_args* args, shivae_s
     SV_REQUIRE(a.V >= 1 && a.V <= SHIVAE_SAMPLE_MAX, "sample_categories: %d categories, 1 to %d are supported", a.V, SHIVAE_SAMPLE_MAX);
     SV_REQUIRE(a.dtype == SHIVAE_F32 || a.dtype == SHIVAE_BF16 || a.dtype == SHIVAE_F16, "sample_categories: unknown dtype %d", a.dtype);
     SV_REQUIRE(a.logits && a.u && a.tokens, "sample_categories: logits, u and tokens are required");
-    const SampleP p{a};
-    SV_BY_DTYPE(a.dtype, launch_sample<E>(p, static_cast<hipStream_t>(stream)));
-    SV_CHECK_HIP(hipGetLastError());
+    // Pieces of the rows whose threads, up to 1024 a row, a launch can have (the choice of threads goes by all rows).
+    constexpr int64_t most = (int64_t)1 << 21;
+    for (int64_t r = 0; r < a.rows; r += most) {
+        SampleP p{a};
+        p.a.logits = static_cast<const char*>(a.logits) + r * a.ld * elem_bytes(a.dtype);
+        p.a.u += r;
+        if (a.temperature_rows) p.a.temperature_rows += r;
+        if (a.top_k_rows) p.a.top_k_rows += r;
+        if (a.top_p_rows) p.a.top_p_rows += r;
+        if (a.min_p_rows) p.a.min_p_rows += r;
+        p.a.tokens += r;
+        if (a.logprob) p.a.logprob += r;
+        p.a.rows = std::min(most, a.rows - r);
+        SV_BY_DTYPE(a.dtype, launch_sample<E>(p, a.rows, static_cast<hipStream_t>(stream)));
+        SV_CHECK_HIP(hipGetLastError());
+    }
     return SHIVAE_OK;
 }

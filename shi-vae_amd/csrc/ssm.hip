@@ -901,16 +901,16 @@ template <class E>
 __global__ __launch_bounds__(256) void ssm_dbc_kernel(SsmP p) {
     const shivae_ssm_args& a = p.a;
     const int64_t rows = (int64_t)a.T * a.B, total = rows * a.G * 2 * a.N;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const int w2 = 2 * a.N, k = (int)(i % w2);
-    const int64_t rg = i / w2, row = rg % rows;
-    const int g = (int)(rg / rows), t = (int)(row / a.B), b = (int)(row - (int64_t)t * a.B);
-    float v = 0.f;
-    if (t < ssm_len(p, b))
-        for (int c = 0; c < p.tiles_g; ++c) v += p.pbc[((int64_t)(g * p.tiles_g + c) * rows + row) * w2 + k];
-    const bool isC = k >= a.N;
-    static_cast<E*>(isC ? a.dC : a.dB)[(row * a.G + g) * a.N + (isC ? k - a.N : k)] = f_elem<E>(v);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int w2 = 2 * a.N, k = (int)(i % w2);
+        const int64_t rg = i / w2, row = rg % rows;
+        const int g = (int)(rg / rows), t = (int)(row / a.B), b = (int)(row - (int64_t)t * a.B);
+        float v = 0.f;
+        if (t < ssm_len(p, b))
+            for (int c = 0; c < p.tiles_g; ++c) v += p.pbc[((int64_t)(g * p.tiles_g + c) * rows + row) * w2 + k];
+        const bool isC = k >= a.N;
+        static_cast<E*>(isC ? a.dC : a.dB)[(row * a.G + g) * a.N + (isC ? k - a.N : k)] = f_elem<E>(v);
+    }
 }
 
 static int ssm_check(const shivae_ssm_args* a, const char* who) {
@@ -1019,14 +1019,15 @@ int shivae_selective_scan_fwd(const shivae_ssm_args* args, void* ws_dev, size_t 
     SV_REQUIRE(a.y, "selective_scan_fwd: y is required");
     SV_REQUIRE(!a.state || a.state != a.state_out || a.T <= TT, "selective_scan_fwd: the state can be updated in place for up to %d rows only", TT);
     ssm_split(p);
-    SV_REQUIRE((int64_t)p.tiles * a.B * p.np < (int64_t)1 << 31, "selective_scan_fwd: B * D is too large");
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a_token(p)) {
         const int V = 4;
         const bool vec = p.E % V == 0 && a.u_sb % V == 0 && a.dt_sb % V == 0 && a.z_sb % V == 0 && a.y_sb % V == 0 && aligned_to(a.u, 16) && aligned_to(a.dt, 16) &&
                          aligned_to(a.z, 16) && aligned_to(a.y, 16) && aligned_to(a.A, 16) && aligned_to(a.state, 16) && aligned_to(a.state_out, 16);
         const int nvec = vec ? a.D / V : a.D;
-        const dim3 grid((unsigned)(((int64_t)a.B * nvec + 255) / 256));
+        const int64_t blocks = ((int64_t)a.B * nvec + 255) / 256;
+        SV_REQUIRE(grid_fits(blocks, 256), "selective_scan_fwd: B * D is too large (%d sequences of %d channel groups)", a.B, nvec);
+        const dim3 grid((unsigned)blocks);
         SV_BY_DTYPE(a.dtype, {
             if (vec) hipLaunchKernelGGL((ssm_token_kernel<E, 4>), grid, dim3(256), 0, s, p, nvec);
             else hipLaunchKernelGGL((ssm_token_kernel<E, 1>), grid, dim3(256), 0, s, p, nvec);
@@ -1034,6 +1035,7 @@ int shivae_selective_scan_fwd(const shivae_ssm_args* args, void* ws_dev, size_t 
         SV_CHECK_HIP(hipGetLastError());
         return SHIVAE_OK;
     }
+    SV_REQUIRE(grid_fits((int64_t)p.tiles * a.B * p.np, 256), "selective_scan_fwd: B * D is too large (%d sequences of %d tiles of 64 channels)", a.B, p.tiles);
     const size_t need = piece_floats(p) * sizeof(float);
     SV_REQUIRE(need == 0 || (ws_dev && ws_bytes >= need && aligned_to(ws_dev, 16)), "selective_scan_fwd: a 16-byte aligned workspace of %zu bytes is needed, not %zu", need, ws_bytes);
     p.hend = static_cast<float*>(ws_dev);
@@ -1064,7 +1066,7 @@ int shivae_selective_scan_bwd(const shivae_ssm_args* args, void* ws_dev, size_t 
     SV_REQUIRE(a.dy && a.du && a.ddt && a.dB && a.dC && a.dA && a.ckpt, "selective_scan_bwd: dy, du, ddt, dB, dC, dA and the forward's ckpt are required");
     SV_REQUIRE((!a.z || a.dz) && (!a.Dp || a.dDp) && (!a.dt_bias || a.ddt_bias), "selective_scan_bwd: z, Dp and dt_bias need buffers for their gradients");
     ssm_split(p);
-    SV_REQUIRE((int64_t)p.tiles * a.B * p.np < (int64_t)1 << 31, "selective_scan_bwd: B * D is too large");
+    SV_REQUIRE(grid_fits((int64_t)p.tiles * a.B * p.np, 256), "selective_scan_bwd: B * D is too large (%d sequences of %d tiles of 64 channels)", a.B, p.tiles);
     const size_t need = bwd_floats(p) * sizeof(float);
     SV_REQUIRE(ws_dev && ws_bytes >= need && aligned_to(ws_dev, 16), "selective_scan_bwd: a 16-byte aligned workspace of %zu bytes is needed, not %zu", need, ws_bytes);
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -1077,8 +1079,7 @@ int shivae_selective_scan_bwd(const shivae_ssm_args* args, void* ws_dev, size_t 
     SV_BY_DTYPE(a.dtype, SV_TRY(launch_ssm_bwd<E>(p, s)));
     SV_CHECK_HIP(hipGetLastError());
     const int64_t total = (int64_t)a.T * a.B * a.G * 2 * a.N;
-    const dim3 grid((unsigned)((total + 255) / 256));
-    SV_REQUIRE((total + 255) / 256 < (int64_t)1 << 31, "selective_scan_bwd: T * B * G * N is too large");
+    const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, 1 << 22));
     SV_BY_DTYPE(a.dtype, hipLaunchKernelGGL((ssm_dbc_kernel<E>), grid, dim3(256), 0, s, p));
     SV_CHECK_HIP(hipGetLastError());
     float* mid = p.pD + (size_t)p.np * a.B * 2 * a.D;
