@@ -987,10 +987,12 @@ template <class E>
 static int launch_ssm_bwd(SsmP& p, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)p.tiles * p.a.B * p.np));
     const int N = p.a.N, S = N <= 4 ? 1 : N <= 8 ? 2 : 4, passes = ceil_div(N, 4 * S);
-    const size_t lds = passes > 1 ? (size_t)passes * 3 * S * 256 * sizeof(float) : 0;  // up to 48 KiB beside 57 of static
+    constexpr size_t pass_lds = 3 * 4 * 256 * sizeof(float), most_lds = 4 * pass_lds;  // N <= 64: up to 48 KiB beside 57 of static
+    const size_t lds = passes > 1 ? passes * pass_lds : 0;
     ssm_vec(p, S);
-    if (lds)  // (past the default limit of 64 KiB)
-        SV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_bwd_kernel<E, 4, true>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (lds)  // (past the default limit of 64 KiB; always to the most, since the limit is the function's and another thread may be between
+              // here and its launch)
+        SV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_bwd_kernel<E, 4, true>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)most_lds));
     if (S == 1) hipLaunchKernelGGL((ssm_bwd_kernel<E, 1, false>), grid, dim3(256), 0, s, p);
     else if (S == 2) hipLaunchKernelGGL((ssm_bwd_kernel<E, 2, false>), grid, dim3(256), 0, s, p);
     else if (passes == 1) hipLaunchKernelGGL((ssm_bwd_kernel<E, 4, false>), grid, dim3(256), 0, s, p);
