@@ -327,6 +327,8 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, 
 
     u, dt, z [T, B, D]; B, C [T, B, G, N], groups of D/G neighbouring channels; A [N, D], D and dt_bias [D] float32, N up to 64;
     initial_state [B, N, D] float32 (None: zeros).  Returns y, or (y, state) with the state behind each sequence's last row.
+    An A of -inf keeps nothing of a state.  NaN stays NaN; what depends on an infinite u or dy is not finite, but may be NaN where the sum
+    above, without the terms that are 0, is an infinity.
     With gradients the states in front of every 16th row are kept (4 N / 16 bytes per element of u) and the rows between are run
     again in the backward pass."""
     u = _first(u, "u", 3)
