@@ -388,7 +388,8 @@ int shivae_selective_scan_bwd(const shivae_ssm_args* args, void* ws_dev, size_t 
  * weight reaches top_p of theirs (>= 1: all), of these the ones with w >= min_p; the largest is always kept.  The token is the
  * first index i, in index order, with sum_{kept j <= i} w_j > u * sum_{kept} w_j; temperature 0 gives the largest logit's
  * index.  NaN logits count as -inf; a row without a logit above -inf gives -1; logits at +inf share everything.  Weights are
- * held as multiples of 2^-43 of the largest (below 2^-44 they are 0), their sums are exact.  No counterpart in the reference
+ * good to 2^-38 of themselves and held as multiples of 2^-43 of the largest (below 2^-44 they are 0); the sums of these are
+ * exact.  No counterpart in the reference
  * (generate_heter_samples averages many draws: shivae_mc_impute). */
 #define SHIVAE_SAMPLE_MAX 1048512
 typedef struct {

@@ -5,7 +5,7 @@
 //   token = the first index i, in index order, with  sum_{kept j <= i} w_j > u * sum_{kept j} w_j
 //
 // Which category is drawn hangs on comparisons of long sums, and 16-bit logits have long runs of equal values, whose errors add up
-// in step.  So a weight is computed in 64 bits (a polynomial for 2^f, error below 2^-38) and held as a multiple of 2^-43 of the
+// in step.  So a weight is computed in 64 bits (a polynomial for 2^f, within 2^-38 of the weight) and held as a multiple of 2^-43 of the
 // largest: sums of these are exact, independent of order (integer LDS atomics included), and fit 63 bits for 2^20 categories.  A
 // weight below 2^-44 of the largest is 0 and is never drawn.  Order is by the logits' own bits, never by rounded quotients.
 //

@@ -37,7 +37,8 @@ def sample_categories(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     The index drawn is the first, in index order, at which the running sum of kept weights exceeds ``u`` times their sum;
     temperature 0 takes the largest logit.  ``u`` [...] float32 holds uniform numbers in [0, 1).  Every setting is a number or a
     tensor [...] with one for each row.  NaN logits count as -inf; a row without a logit above -inf gives -1; logits at +inf share
-    everything.  Sums are exact (weights are held to 2^-43 of the largest), so the result does not depend on scheduling.
+    everything.  A weight is good to 2^-38 of itself and held as a multiple of 2^-43 of the largest (0 below 2^-44); sums of these are exact,
+    so the result does not depend on scheduling.
 
     Returns int64 indices [...], or (indices, log-probability of the index among the kept [...] float32); the log-probability
     is 0 for temperature 0 and -inf where the index is -1.  It has no derivative: with logits or a temperature that require one the call
