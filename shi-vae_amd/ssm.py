@@ -230,7 +230,7 @@ def causal_conv_step(x, weight, bias=None, *, state, activation=None, state_out=
     weight, bias = _conv_params(weight, bias, D, dev)
     _activation(state, "state", (weight.shape[0] - 1, B, D), x.dtype, dev)
     out, state = _step_state(state, state_out), state.contiguous()
-    _no_backward(x, weight, bias, state)
+    _no_backward(x, weight, bias, state, out)
     y = torch.empty((B, D), dtype=x.dtype, device=dev)
     args = N.ConvArgs(1, B, D, weight.shape[0], _DTYPES[x.dtype], _conv_silu(activation), x.data_ptr(), 0, x.stride(0), weight.data_ptr(),
                       _ptr(bias), state.data_ptr(), None, y.data_ptr(), 0, D, out.data_ptr())
@@ -350,7 +350,7 @@ def selective_scan_step(u, dt, A, B, C, state, D=None, z=None, dt_bias=None, sof
     dt, A, B, C, D, z, dt_bias = _scan_inputs(u, dt, A, B, C, D, z, dt_bias)
     _activation(state, "state", (Bt, A.shape[0], Dm), torch.float32, dev)
     out, state = _step_state(state, state_out), state.contiguous()
-    _no_backward(u, dt, A, B, C, D, z, dt_bias, state)
+    _no_backward(u, dt, A, B, C, D, z, dt_bias, state, out)
     y = torch.empty((Bt, Dm), dtype=u.dtype, device=dev)
     args = N.SsmArgs(1, Bt, Dm, A.shape[0], B.shape[1], _DTYPES[u.dtype], int(bool(softplus)), u.data_ptr(), dt.data_ptr(), _ptr(z), 0,
                      u.stride(0), 0, dt.stride(0), 0, 0 if z is None else z.stride(0), B.data_ptr(), C.data_ptr(), 0, B.stride(0),

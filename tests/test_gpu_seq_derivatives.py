@@ -80,3 +80,15 @@ def test_the_log_probability_is_not_differentiable():
     with forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             f(forward_ad.make_dual(lg, torch.ones_like(lg)), u, t, return_logprob=True)
+
+
+def test_a_new_state_that_requires_a_gradient_is_refused():
+    """As an in-place write to a leaf is; under no_grad it is written."""
+    for f, kw in _calls()[1::2]:
+        out = torch.zeros_like(kw["state"]).requires_grad_(True)
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            f(**kw, state_out=out)
+        assert not out.any()
+        with torch.no_grad():
+            f(**kw, state_out=out)
+        assert out.any()
