@@ -46,16 +46,13 @@ __device__ __forceinline__ int ssm_len(const SsmP& p, int b) {
 }
 
 // A log2(e), infinities made finite: an A of -inf (no memory) has to give exp(0 A) = 1 behind a sequence's end, and 0 where a step is
-// positive.  A NaN stays one (comparisons, since fminf and fmaxf return the other operand).
-__device__ __forceinline__ float scale_A(float A) {
-    const float v = A * kLog2e;
-    return v < -3.4e38f ? -3.4e38f : (v > 3.4e38f ? 3.4e38f : v);
-}
+// positive.  A NaN stays one (v_maximum3_f32; fminf and fmaxf return the other operand).
+__device__ __forceinline__ float scale_A(float A) { return __builtin_elementwise_minimum(__builtin_elementwise_maximum(A * kLog2e, -3.4e38f), 3.4e38f); }
 
 // 2^x v + add, where 2^x alone may leave the range of fp32: x is the sum of a piece's log2 decays, and decays that grow (s A > 0) take a
 // state of 0, or a small one, through a piece without ever leaving the range.
 __device__ __forceinline__ float decay_add(float x, float v, float add) {
-    const float k = fabsf(x) <= 126.f ? 0.f : rintf(fminf(fmaxf(x, -1e4f), 1e4f)), f = (x > 1e4f ? 1e4f : x) - k;
+    const float k = fabsf(x) <= 126.f ? 0.f : rintf(fminf(fmaxf(x, -1e4f), 1e4f)), f = __builtin_elementwise_minimum(x, 1e4f) - k;
     return fmaf(__builtin_amdgcn_exp2f(f), __builtin_amdgcn_ldexpf(v, (int)k), add);
 }
 
@@ -207,6 +204,31 @@ __device__ __forceinline__ void unroll(F f) {  // f(0), f(1), ... with the numbe
     [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
 }
 
+// What the pieces hand on to each other, S states of a lane's channel at a time (states at and behind N are read as the last one).
+template <int S>
+struct PieceStates {
+    const SsmP& p;
+    const float *hend, *ssum;  // of this sequence and channel
+    int s0;
+    __device__ __forceinline__ PieceStates(const SsmP& p, const Place& q, int s0)
+        : p(p), hend(p.hend + (int64_t)q.b * p.a.N * p.a.D + q.d), ssum(p.ssum + (int64_t)q.b * p.a.D + q.d), s0(s0) {}
+    __device__ __forceinline__ const float* state(int c, int j) const { return hend + ((int64_t)c * p.a.B * p.a.N + min(s0 + j, p.a.N - 1)) * p.a.D; }
+    __device__ __forceinline__ void load(float (&v)[S], int c) const {
+#pragma unroll
+        for (int j = 0; j < S; ++j) v[j] = *state(c, j);
+    }
+    // v through piece c: prod_t exp(s_t A) = exp(A sum_t s_t), and what the piece itself left.
+    __device__ __forceinline__ void pass(float (&v)[S], const float (&A2)[S], int c) const {
+        const float sum = ssum[(int64_t)c * p.a.B * p.a.D];
+#pragma unroll
+        for (int j = 0; j < S; ++j) v[j] = decay_add(A2[j] * sum, v[j], *state(c, j));
+    }
+    __device__ __forceinline__ void clear(float (&v)[S], bool ok) const {
+#pragma unroll
+        for (int j = 0; j < S; ++j) v[j] = ok && s0 + j < p.a.N ? v[j] : 0.f;
+    }
+};
+
 // A wave owns 16 channels: lane = (state group g4 = lane / 16, channel lane % 16), S states of the channel per lane.  Of a tile's 16
 // rows the lane prepares row 4 k + g4 for its channel (k = 0..3: softplus, s u, later the gate and the store), so that this work is done
 // once per channel; the state groups get s and s u through the wave's own 2 KiB of LDS, and y's parts come back summed, row 4 k + g4 in
@@ -231,13 +253,12 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
         const int64_t o = state0 + (int64_t)j * a.D;
         A2[j] = live ? scale_A(a.A[(int64_t)(g4 * S + j) * a.D + q.d]) : 0.f;
         h[j] = live && q.piece == 0 && a.state ? a.state[o] : 0.f;
-        if (!FIRST && live && q.piece) {
-            h[j] = p.hend[o];
-            for (int c = 1; c < min(q.piece, pieces); ++c) {
-                const float sum = p.ssum[((int64_t)c * a.B + q.b) * a.D + q.d];
-                h[j] = decay_add(A2[j] * sum, h[j], p.hend[c * statep + o]);
-            }
-        }
+    }
+    if (!FIRST && q.piece) {
+        PieceStates<S> in(p, q, g4 * S);
+        in.load(h, 0);
+        for (int c = 1; c < min(q.piece, pieces); ++c) in.pass(h, A2, c);
+        in.clear(h, q.ok);
     }
     const float bias = a.dt_bias ? a.dt_bias[q.d] : 0.f, Dp = (!FIRST && a.Dp) ? a.Dp[q.d] : 0.f;
     const unsigned le = q.lo * (unsigned)sizeof(E);
@@ -424,16 +445,20 @@ __global__ __launch_bounds__(256) void ssm_token_kernel(SsmP p, int nvec) {
     *reinterpret_cast<Pack<E, V>*>(static_cast<E*>(a.y) + (int64_t)b * a.y_sb + d) = ry;
 }
 
-// Where the adjoint of a piece's last state comes from: the gradient of state_out for the last piece, otherwise what the pieces behind
-// it hand down (prod_t exp(s_t A) = exp(A sum_t s_t), as in the forward pass).
-__device__ __forceinline__ float piece_adjoint(const SsmP& p, const Place& q, int n, int s, float A2) {
+// The adjoint of a piece's last state: the gradient of state_out for the last piece, otherwise what the pieces behind it hand down (those
+// behind the sequence's end what they get).
+template <int S>
+__device__ __forceinline__ void piece_adjoints(const SsmP& p, const Place& q, int n, int s0, const float (&A2)[S], float (&v)[S]) {
     const shivae_ssm_args& a = p.a;
-    const int64_t o = ((int64_t)q.b * a.N + s) * a.D + q.d;
-    if (q.piece == p.np - 1) return a.dstate_out ? a.dstate_out[o] : 0.f;
-    float v = p.hend[(int64_t)(p.np - 1) * a.B * a.N * a.D + o];
-    for (int c = min(p.np - 1, (n + p.plen - 1) / p.plen) - 1; c > q.piece; --c)  // (pieces behind the sequence's end hand on what they get)
-        v = decay_add(A2 * p.ssum[((int64_t)c * a.B + q.b) * a.D + q.d], v, p.hend[(int64_t)c * a.B * a.N * a.D + o]);
-    return v;
+    PieceStates<S> in(p, q, s0);
+    if (q.piece == p.np - 1) {
+#pragma unroll
+        for (int j = 0; j < S; ++j) v[j] = a.dstate_out ? a.dstate_out[((int64_t)q.b * a.N + min(s0 + j, a.N - 1)) * a.D + q.d] : 0.f;
+    } else {
+        in.load(v, p.np - 1);
+        for (int c = min(p.np - 1, (n + p.plen - 1) / p.plen) - 1; c > q.piece; --c) in.pass(v, A2, c);
+    }
+    in.clear(v, q.ok);
 }
 
 // The operands of the backward kernels: 16-row tiles from a piece's last to its first, requested a tile ahead.
@@ -658,15 +683,17 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
             const int s = k * P + g4 * S + j;
             const bool live = q.ok && s < a.N;
             A2[j] = live ? scale_A(a.A[(int64_t)s * a.D + q.d]) : 0.f;
-            ag[j] = live ? piece_adjoint(p, q, n, s, A2[j]) : 0.f;
             dA[j] = 0.f;
-            if (MANY) {
+        }
+        piece_adjoints<S>(p, q, n, k * P + g4 * S, A2, ag);
+        if (MANY)
+#pragma unroll
+            for (int j = 0; j < S; ++j) {
                 float* o = kept + (int64_t)k * 3 * S * 256 + threadIdx.x;
                 o[j * 256] = ag[j];
                 o[(S + j) * 256] = A2[j];
                 o[(2 * S + j) * 256] = 0.f;
             }
-        }
     }
     const float bias = a.dt_bias ? a.dt_bias[q.d] : 0.f, Dp = a.Dp ? a.Dp[q.d] : 0.f;
     const int64_t last = t0 < tn ? (tn - 1) / TT * TT : t0, statep = (int64_t)a.B * a.N * a.D;
