@@ -9,7 +9,7 @@
 // largest: sums of these are exact, independent of order (integer LDS atomics included), and fit 63 bits for 2^20 categories.  A
 // weight below 2^-44 of the largest is 0 and is never drawn.  Order is by the logits' own bits, never by rounded quotients.
 //
-// Measured (us): 256 x 131072, bf16, top-p 0.95 133, with min-p 0.01 115, top-k 50 35, no cut 62, the largest alone 24; 1 x 32768, top-k 50
+// Measured (us): 256 x 131072, bf16, top-p 0.95 133, with min-p 0.01 114, top-k 50 35, no cut 62, the largest alone 24; 1 x 32768, top-k 50
 // 14, with top-p 15.6; 102400 rows of 8 9.  Where it hurts: a row stays on one compute unit, 1 x 131072 with top-p takes 118 us.
 //
 // A row is a workgroup's.  No row is sorted: top-k and top-p need the last element they keep.  A histogram of (max - x) /
@@ -715,7 +715,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleP p) {
 // ------------------------------------------------------------------------------------------------ few categories
 // L lanes per row (a power of two), a lane per category.  A lane finds what precedes it in the order by looking at every other one.
 // 16384 rows of 60, top-p: 32 us, against 46 by a workgroup of one wave for each (44 with exchanges through LDS instead of v_readlane);
-// of 24: 14.5 against 35.
+// of 24: 14.5 against 35.  102400 rows of 8, no cut: 8.6, of which 284 vector instructions a wave (8 rows) take 5.9 to issue; the
+// log-probability's logarithm in 64 bits is 2.4 of the 8.6.  With top-p 10.3.
 template <class E, int L>
 __global__ __launch_bounds__(256) void sample_few_kernel(SampleP p) {
     const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;

@@ -12,8 +12,9 @@
 // (one cache line of bf16).  Rows come in tiles of 16, requested a tile ahead.  Where B * D is small the time axis is split into pieces: a
 // first launch runs each piece from a zero state and keeps its last state and sum of s; since prod_t exp(s_t A) = exp(A sum_t s_t), a piece
 // of the second launch gets its first state from those of the pieces in front of it (backward: the adjoint from those behind).
-// Measured (MI355X, us): T 2048, B 16, D 2048, N 16, bf16, gate: 350 (1.55 TB/s); at B 64 1095, 245 G pairs a second, 0.75 of the bound: at
-// B 16 a SIMD has two waves, whose dependent exponentials are not covered.  T 8192, B 1: 150 in 32 pieces; in 16 pieces 167.
+// Measured (MI355X, us a call, GPU time of captured calls): T 2048, B 16, D 2048, N 16, bf16, gate: 328 (1.65 TB/s); at B 64 1057, 254 G
+// pairs a second, 0.78 of the bound: at B 16 a SIMD has two waves, whose dependent exponentials are not covered.  T 8192, B 1: 139 in 32
+// pieces; in 16 pieces 151.  With 32 and 64 states: 502 and 1004; T 8192, B 1 with 64 539.
 // Earlier forms of the same kernel, at B 16: 64 channels a wave and the states over four waves, s, B and C from LDS: 404 (64 of its 96 LDS
 // cycles per row were broadcasts of B and C); B and C by scalar loads: 757; by row_newbcast: 415; waves that share nothing: 350.
 #include <algorithm>
@@ -397,8 +398,8 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(SsmP p) {
 }
 
 // One row.  A thread owns V neighbouring channels of one sequence and walks the states: the fp32 state is read and written
-// once, 16 bytes a lane, and is nearly all of the traffic: B 256, D 2048, N 16, bf16: 16.4 us for 67 MB of
-// it, 4.1 TB/s.
+// once, 16 bytes a lane, and is nearly all of the traffic: B 256, D 2048, N 16, bf16: 17 us for 67 MB of it, 3.9 TB/s; with 64 states 52.
+// Channels that are not 16-byte aligned, one a thread, cost nothing: slices 8 bytes off 16 us, D 2046 17.
 template <class E, int V>
 __global__ __launch_bounds__(256) void ssm_token_kernel(SsmP p, int nvec) {
     const shivae_ssm_args& a = p.a;
@@ -653,9 +654,10 @@ __device__ __forceinline__ Sums<S> sum_rows(F& f, int lane) {
 // with states and decays in registers (128 of them for S = 4), then back.  More than 16 states take several passes over a tile, 4 S
 // states each, whose adjoints and sums wait in LDS.  dB and dC are sums over all channels: of the wave's 16 by sum_rows, of the
 // workgroup's four waves through LDS (the one barrier of a pass), of the workgroups by ssm_dbc_kernel.
-// Bound by vector instructions: 197 us (T 2048, B 4, D 1536, N 16, bf16, gate, 10 pieces), in which a SIMD issues 7.7e4 of them, 0.65 of its
-// time; 218 us (T 1000, B 64, D 256, fp32).  The four passes around it: ssm_fwd_kernel 50 (FIRST) and 71, ssm_bwd_first_kernel 47,
-// ssm_dbc_kernel 10.  The sums over channels by LDS atomics on floats instead (200 cycles each) took longer than all of the rest.
+// Bound by vector instructions: 206 us (T 2048, B 4, D 1536, N 16, bf16, gate, 10 pieces), in which a SIMD issues 7.7e4 of them, 0.63 of its
+// time; 222 us (T 1000, B 64, D 256, fp32).  The four passes around it: ssm_fwd_kernel 52 (FIRST) and 72, ssm_bwd_first_kernel 48,
+// ssm_dbc_kernel 10 (all from a trace of 13 calls; a long run of calls takes 372 for all, 0.94 of their sum).  With 32 and 64 states, two
+// and four passes over a tile: 777 and 1974 forward and backward.  The sums over channels by LDS atomics on floats instead (200 cycles each) took longer than all of the rest.
 template <class E, int S, bool MANY>
 __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
     constexpr int P = 4 * S;  // states of a pass
@@ -956,9 +958,9 @@ static int ssm_check(const shivae_ssm_args* a, const char* who) {
 
 // Pieces of the time axis.  A split costs the second launch's work again without y (0.7 of it; backward a quarter), so it is taken only
 // up to 256 workgroups, one wave a SIMD: then pieces of at least 64 rows until there are about 1024.  Measured (us, forward and backward
-// together): T 1000, B 64, D 256, fp32, 256 workgroups: split 420, not 471; T 2048, B 4, D 1536, bf16, 96 workgroups: split 385, not 932.
-// For 512 / 1024 / 1536 / 2048 workgroups: T 8192, B 1, D 2048 forward 167 / 158 / 158 / 160; the two above 427 / 421 / 416 / 424 and
-// 398 / 385 / 380 / 400.
+// together): T 1000, B 64, D 256, fp32, 256 workgroups: split 408, not 471; T 2048, B 4, D 1536, bf16, 96 workgroups: split 372, not 932.
+// For 512 / 1024 / 1536 / 2048 workgroups (up to 64 pieces in the last): T 8192, B 1, D 2048 forward 151 / 139 / 141 / 154; the two above
+// 417 / 408 / 396 / 397 and 390 / 372 / 357 / 372.
 static void ssm_split(SsmP& p) {
     const shivae_ssm_args& a = p.a;
     p.E = a.D / a.G;
