@@ -657,7 +657,8 @@ __device__ __forceinline__ Sums<S> sum_rows(F& f, int lane) {
 // Bound by vector instructions: 206 us (T 2048, B 4, D 1536, N 16, bf16, gate, 10 pieces), in which a SIMD issues 7.7e4 of them, 0.63 of its
 // time; 222 us (T 1000, B 64, D 256, fp32).  The four passes around it: ssm_fwd_kernel 52 (FIRST) and 72, ssm_bwd_first_kernel 48,
 // ssm_dbc_kernel 10 (all from a trace of 13 calls; a long run of calls takes 372 for all, 0.94 of their sum).  With 32 and 64 states, two
-// and four passes over a tile: 777 and 1974 forward and backward.  The sums over channels by LDS atomics on floats instead (200 cycles each) took longer than all of the rest.
+// and four passes over a tile: 777 and 1974 forward and backward.  The sums over channels by LDS atomics on floats instead (200 cycles each)
+// took longer than all of the rest.
 template <class E, int S, bool MANY>
 __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(SsmP p) {
     constexpr int P = 4 * S;  // states of a pass
